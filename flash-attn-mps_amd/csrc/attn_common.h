@@ -66,10 +66,33 @@ FA_DEV float descale_of(const float* p, const int64_t* st, int64_t b, int kh) {
   return p ? p[b * st[0] + (int64_t)kh * st[1]] : 1.0f;
 }
 
+// Kernel arguments of attention over a block-scaled cache (fa_block_attn_args
+// with 32-bit block counts): the attention's own, and the E8M0 scales.
+struct fa_block_attn : fa_attn_args {
+  const uint8_t* scale[2];      // K, V
+  int64_t scale_stride[2][3];   // page, block, head
+  int32_t block;                // tokens per scale
+};
+
+template <bool BLOCK> struct AttnArgsOf { using type = fa_attn_args; };
+template <> struct AttnArgsOf<true> { using type = fa_block_attn; };
+
+// 2^(e - 127) of an E8M0 byte (e = 255: NaN).
+FA_DEV float e8m0_to_f32(uint32_t e) {
+  return __uint_as_float(e == 0 ? 0x00400000u : e == 255 ? 0x7fc00000u : e << 23);
+}
+
+// Scale byte of head kh for the key at row `row` of page `page` (V: which = 1).
+FA_DEV uint32_t scale_byte(const fa_block_attn& a, int which, int64_t page, int row, int kh) {
+  const int64_t* st = a.scale_stride[which];
+  return a.scale[which][page * st[0] + (int64_t)(row / a.block) * st[1] + (int64_t)kh * st[2]];
+}
+
 // The arguments with window bounds of 2^30 and more (past any two positions'
 // distance) as -1, unbounded: the kernels add bounds to positions in 32 bits.
-inline fa_attn_args fa_bounded(const fa_attn_args& args) {
-  fa_attn_args a = args;
+template <typename A>
+inline A fa_bounded(const A& args) {
+  A a = args;
   if (a.window_left >= 1 << 30) a.window_left = -1;
   if (a.window_right >= 1 << 30) a.window_right = -1;
   return a;
@@ -77,6 +100,10 @@ inline fa_attn_args fa_bounded(const fa_attn_args& args) {
 
 // Host-side argument checks shared by fa_attn_fwd / fa_decode_fwd / fa_prefill_fwd.
 int fa_validate_attn(const fa_attn_args* a, const char* who);
+
+// The checks of a block-scaled call, and its kernel arguments in `out` (window
+// bounds as fa_bounded gives them).
+int fa_validate_block(const fa_block_attn_args* args, fa_block_attn* out, const char* who);
 
 // fa_merge_partials for the splits of one call: a NaN LSE makes the row NaN,
 // with LSE -inf, as one split would (fp32 rows over at most 256 dims).

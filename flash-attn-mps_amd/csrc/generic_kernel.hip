@@ -10,7 +10,7 @@
 // owning output dimensions.  A row's result depends only on that row's data
 // and its split range, never on the rest of the batch, so num_splits == 1 is
 // batch-invariant (flash_attn_mps/tests/test_vllm.py:152-159).
-#include "attn_common.h"
+#include "block_row.h"
 
 namespace {
 
@@ -114,6 +114,35 @@ __global__ __launch_bounds__(256) void attn_generic_kernel(const fa_attn_args a)
   }
 }
 
+// Block-scaled caches: the same grid and splits, a row by block_row.
+__global__ __launch_bounds__(256) void attn_block_kernel(const fa_block_attn a) {
+  __shared__ float q_smem[GEN_WAVES][GEN_MAX_D];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int64_t S = a.num_splits;
+  const int64_t b = blockIdx.z / S, split = blockIdx.z - (blockIdx.z / S) * S;
+  const int h = blockIdx.y, kh = h / (int)(a.heads_q / a.heads_k);
+  const int qi = blockIdx.x * GEN_WAVES + wave;
+  const RequestInfo r = load_request(a, b);
+  if (qi >= r.q_len) return;   // (each wave uses its own row of q_smem)
+  const int64_t tq = (int64_t)r.q_begin + qi;
+  float* const qrow = q_smem[wave];
+  for (int d = lane; d < (int)a.head_dim_qk; d += 64)
+    qrow[d] = load_any(a.q, tq * a.q_stride[0] + (int64_t)h * a.q_stride[1] + d * a.q_stride[2], a.q_dtype);
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+  const int begin = (int)((int64_t)r.k_len * split / S), end = (int)((int64_t)r.k_len * (split + 1) / S);
+  const float lse = block_row<GEN_MAX_D / 64>(
+      a, b, r, kh, h, (int)split, tq, qi + r.k_len - r.q_len, begin, end, lane, [&](int d) { return qrow[d]; },
+      [&](int d, float x) {
+        if (S == 1) store_any(a.out, tq * a.out_stride[0] + (int64_t)h * a.out_stride[1] + d * a.out_stride[2], a.out_dtype, x);
+        else a.partial_out[((split * a.total_q + tq) * a.heads_q + h) * a.head_dim_v + d] = x;
+      });
+  if (lane != 0) return;
+  if (S == 1) a.lse[(int64_t)h * a.lse_stride[0] + tq * a.lse_stride[1]] = lse != lse ? -INFINITY : lse;
+  else a.partial_lse[(split * a.heads_q + h) * a.total_q + tq] = lse;
+}
+
 template <typename KT>
 int launch_generic_v(const fa_attn_args& a, dim3 grid, hipStream_t s) {
   switch (a.v_dtype) {
@@ -147,17 +176,65 @@ int fa_validate_attn(const fa_attn_args* a, const char* who) {
   return FA_OK;
 }
 
+int fa_validate_block(const fa_block_attn_args* args, fa_block_attn* out, const char* who) {
+  FA_REQUIRE(args && args->size == (int64_t)sizeof(fa_block_attn_args), "%s: null or mismatched arguments", who);
+  const fa_attn_args& a = args->attn;
+  const int rc = fa_validate_attn(&a, who);
+  if (rc) return rc;
+  FA_REQUIRE(a.k_dtype == FA_E4M3 && a.v_dtype == FA_E4M3 && a.page_size > 0 && a.seqused_k && !a.leftpad_k,
+             "%s: block scales go with a paged E4M3 cache", who);
+  FA_REQUIRE(!a.k_descale && !a.v_descale, "%s: block scales take the place of descales", who);
+  FA_REQUIRE(!a.k || (args->k_scale && args->v_scale), "%s: null scales", who);
+  FA_REQUIRE(args->block >= 1 && args->block <= a.page_size && a.page_size % args->block == 0 && a.page_size <= INT32_MAX,
+             "%s: a block must divide the page size", who);
+  static_cast<fa_attn_args&>(*out) = fa_bounded(a);
+  out->scale[0] = args->k_scale, out->scale[1] = args->v_scale;
+  for (int i = 0; i < 3; ++i) {
+    out->scale_stride[0][i] = args->k_scale_stride[i];
+    out->scale_stride[1][i] = args->v_scale_stride[i];
+  }
+  out->block = (int32_t)args->block;
+  return FA_OK;
+}
+
+namespace {
+
+int generic_checks(const fa_attn_args* a, const char* who) {
+  FA_REQUIRE(a->num_splits == 1 || (a->partial_out && a->partial_lse), "%s: splits need partial buffers", who);
+  FA_REQUIRE(a->max_seqlen_q >= 1, "%s: max_seqlen_q must be positive", who);
+  FA_REQUIRE(a->batch * a->num_splits <= 65535, "%s: batch*splits exceeds the grid limit", who);
+  FA_REQUIRE(a->heads_q <= 65535, "%s: too many heads", who);
+  return FA_OK;
+}
+
+dim3 generic_grid(const fa_attn_args* a) {
+  return dim3((unsigned)fa_ceil_div(a->max_seqlen_q, GEN_WAVES), (unsigned)a->heads_q,
+              (unsigned)(a->batch * a->num_splits));
+}
+
+int generic_merge(const fa_attn_args* a, void* stream);
+
+}  // namespace
+
+extern "C" int fa_block_attn_fwd(const fa_block_attn_args* args, void* stream) {
+  fa_block_attn a;
+  int rc = fa_validate_block(args, &a, "fa_block_attn_fwd");
+  if (rc || a.total_q == 0) return rc;
+  rc = generic_checks(&a, "fa_block_attn_fwd");
+  if (rc) return rc;
+  hipLaunchKernelGGL(attn_block_kernel, generic_grid(&a), dim3(256), 0, (hipStream_t)stream, a);
+  rc = fa_check_launch("fa_block_attn_fwd");
+  return rc || a.num_splits == 1 ? rc : generic_merge(&a, stream);
+}
+
 extern "C" int fa_attn_fwd(const fa_attn_args* args, void* stream) {
   int rc = fa_validate_attn(args, "fa_attn_fwd");
   if (rc) return rc;
   const fa_attn_args bounded = fa_bounded(*args), *a = &bounded;
   if (a->total_q == 0) return FA_OK;
-  FA_REQUIRE(a->num_splits == 1 || (a->partial_out && a->partial_lse), "fa_attn_fwd: splits need partial buffers");
-  FA_REQUIRE(a->max_seqlen_q >= 1, "fa_attn_fwd: max_seqlen_q must be positive");
-  FA_REQUIRE(a->batch * a->num_splits <= 65535, "fa_attn_fwd: batch*splits exceeds the grid limit");
-  FA_REQUIRE(a->heads_q <= 65535, "fa_attn_fwd: too many heads");
-  const dim3 grid((unsigned)fa_ceil_div(a->max_seqlen_q, GEN_WAVES), (unsigned)a->heads_q,
-                  (unsigned)(a->batch * a->num_splits));
+  rc = generic_checks(a, "fa_attn_fwd");
+  if (rc) return rc;
+  const dim3 grid = generic_grid(a);
   hipStream_t s = (hipStream_t)stream;
   // fp32 at the matrix-core kernel's head dims and alignment (any feature):
   // dense causal 2 x 1024 tokens, 16/8 heads, d128 4940 us here.
@@ -171,7 +248,12 @@ extern "C" int fa_attn_fwd(const fa_attn_args* args, void* stream) {
       default: rc = launch_generic_v<F32T>(*a, grid, s); break;
     }
   }
-  if (rc || a->num_splits == 1) return rc;
+  return rc || a->num_splits == 1 ? rc : generic_merge(a, stream);
+}
+
+namespace {
+
+int generic_merge(const fa_attn_args* a, void* stream) {
   fa_merge_partials_args m;
   m.partial = a->partial_out;
   m.partial_lse = a->partial_lse;
@@ -194,3 +276,5 @@ extern "C" int fa_attn_fwd(const fa_attn_args* args, void* stream) {
   for (int i = 0; i < 2; ++i) m.lse_stride[i] = a->lse_stride[i];
   return fa_merge_splits(&m, stream);
 }
+
+}  // namespace

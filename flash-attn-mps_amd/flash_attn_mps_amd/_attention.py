@@ -28,6 +28,7 @@ kernel variant depends only on dtypes, head dims and feature flags, and a
 key tile that a row cannot see adds exact zeros to its sums.  So a request's
 rows are bit-identical whatever else is in the batch.
 """
+import ctypes
 import math
 
 import torch
@@ -109,8 +110,30 @@ def build_args(p, out, lse, max_q=None):
         causal, _bound(window_left), _bound(window_right), kind, mask_window, mask_clamp, *flags,
         *ranges, *prefix, window_len,
         q_shape[2] ** -0.5 if p.scale is None else _float32(p.scale), _float32(p.softcap),
-        *alibi, *vector(p.sinks, f32), *matrix(p.q_descale, f32), *matrix(p.k_descale, f32), *matrix(p.v_descale, f32),
+        *alibi, *vector(p.sinks, f32), *matrix(p.q_descale, f32),
+        *((0,) * 6 if p.block_scaled else (*matrix(p.k_descale, f32), *matrix(p.v_descale, f32))),
         1, 0, 0, 0, 0, 0)
+
+
+def _entry(p, name, a):
+    """The entry point `name` and its arguments for Problem `p`: a block-scaled
+    cache has its own (fa_block_*), with the scales beside the attention's."""
+    if not p.block_scaled:
+        return name, a
+    k, v = p.k_descale, p.v_descale
+    block = _lib.BlockAttnArgs(ctypes.sizeof(_lib.BlockAttnArgs), a, k.data_ptr(), v.data_ptr(), k.stride(), v.stride(),
+                               p.k.shape[1] // k.shape[1])
+    return name.replace("fa_", "fa_block_", 1), block
+
+
+def call(p, name, a):
+    """The entry point `name` on Problem `p`'s device."""
+    name, args = _entry(p, name, a)
+    _lib.call(name, args, p.device)
+
+
+def supported(p, name, a):
+    return _lib.supported(*_entry(p, name, a))
 
 
 def _fits_prefill(p, out):
@@ -351,6 +374,8 @@ def solve(p):
         raise ValueError("nonempty queries need max_seqlen_q >= 1")
     if p.batch < 1:
         raise ValueError("cu_seqlens_q needs at least two offsets")
+    if p.block_scaled:
+        return _solve_generic(p, out)
     if p.max_q == 1 and not p.deterministic and p.mask is None:
         from ._decode import decode
         return decode(p, out)
@@ -393,4 +418,12 @@ def solve(p):
         _partials(p, a, (splits, p.tokens, p.heads, p.dim_v), (splits, p.heads, p.tokens))
     a.num_splits = splits
     _lib.call("fa_attn_fwd", a, p.device)
+    return out, lse
+
+
+def _solve_generic(p, out):
+    lse = torch.empty((p.heads, p.tokens), device=p.device, dtype=torch.float32)
+    a = build_args(p, out, lse)
+    a.num_splits = 1
+    call(p, "fa_attn_fwd", a)
     return out, lse

@@ -8,6 +8,10 @@ flash_attn_mps/_cache.py:55-155).
   or through a page table; the lengths themselves are not touched.
 * rotary_append is a generation step's rotary embedding and append in one
   launch.
+* rotary_embedding turns packed rows by positions on one to four axes, and
+  append_paged_kvcache writes packed rows of requests to a paged cache with that
+  rotation on the way; its E4M3 caches may hold a power of two per block of
+  tokens and head (E8M0) in place of a scale per head.
 * An FP8 (E4M3FN) cache stores E4M3(x / scale) with scale a scalar or one
   value per KV head; 16-bit and fp32 caches of the input's dtype get the
   input's bits.
@@ -18,9 +22,28 @@ from functools import lru_cache
 import torch
 
 from . import _lib
-from ._problem import on_gpu
+from ._problem import Want, on_gpu, reject_training
 
 _INPUT_TYPES = (torch.float16, torch.bfloat16, torch.float32)
+BLOCK_SCALE = torch.float8_e8m0fnu
+
+
+def is_block_scale(scale):
+    """Whether `scale` is the scales of a block-scaled cache (E8M0, a power of two per block and head)."""
+    return torch.is_tensor(scale) and scale.dtype == BLOCK_SCALE
+
+
+def block_of(cache, scale, name):
+    """Tokens per scale of a paged E4M3 cache [pages, P, H, D] whose scales [pages, P / block, H] are `scale`."""
+    if cache.ndim != 4 or cache.dtype != torch.float8_e4m3fn:
+        raise TypeError(f"{name} goes with a paged float8_e4m3fn cache")
+    pages, size, heads = cache.shape[:3]
+    if scale.ndim != 3 or scale.shape[0] != pages or scale.shape[2] != heads or not scale.shape[1] \
+            or size % scale.shape[1]:
+        raise ValueError(f"{name} {tuple(scale.shape)} must be [{pages}, blocks dividing {size}, {heads}]")
+    if scale.device != cache.device:
+        raise ValueError(f"{name} is on {scale.device}; expected the cache's device {cache.device}")
+    return size // scale.shape[1]
 
 
 def _require_gpu(**tensors):
@@ -37,6 +60,8 @@ def _one(device):
 
 def _per_head_scale(scale, heads, device):
     """(fp32 tensor, stride): stride 0 shares one scale, 1 reads one per head."""
+    if is_block_scale(scale):
+        raise TypeError("scales per block (float8_e8m0fnu) go with append_paged_kvcache")
     t = _one(device) if scale is None else torch.as_tensor(scale, dtype=torch.float32, device=device)
     if t.numel() == 1:
         return t.reshape(1), 0
@@ -255,3 +280,159 @@ def rotary(q, k, cos, sin, cache_seqlens, *, rotary_interleaved=True, causal=Fal
             _lib.call("fa_rotary", a, x.device)
         rotated.append(y)
     return tuple(rotated)
+
+
+@lru_cache(maxsize=64)
+def _pair_axis_words(pair_axes, half, axes):
+    """The axis of each rotated pair, two bits a pair in eight 64-bit words."""
+    if pair_axes is None:
+        if axes > 1:
+            raise ValueError(f"positions on {axes} axes need pair_axes, the axis of each of the {half} rotated pairs")
+        return (0,) * 8
+    if len(pair_axes) != half or any(type(a) is not int or not 0 <= a < axes for a in pair_axes):
+        raise ValueError(f"pair_axes must hold one axis in 0..{axes - 1} for each of the {half} rotated pairs")
+    words = [0] * 8
+    for i, a in enumerate(pair_axes):
+        words[i >> 5] |= a << (2 * (i & 31))
+    return tuple(words)
+
+
+_NO_ROTATION = (0,) * 23
+
+
+def _rotation(cos, sin, positions, pair_axes, interleaved, tokens, dims, device):
+    """The fa_rotation fields of a checked rotation of rows with head dims `dims`."""
+    if cos.ndim != 2 or sin.shape != cos.shape or sin.dtype != cos.dtype:
+        raise ValueError(f"rotary_cos {tuple(cos.shape)} and rotary_sin {tuple(sin.shape)} must be one "
+                         "[positions, rotary_dim / 2] and one type")
+    if cos.dtype not in _INPUT_TYPES:
+        raise TypeError(f"rotary tables are float16, bfloat16 or float32; got {cos.dtype}")
+    if cos.device != device or sin.device != device:
+        raise ValueError(f"rotary tables on {cos.device} / {sin.device}; expected {device}")
+    rows, half = cos.shape
+    if 2 * half > min(dims):
+        raise ValueError(f"rotary_dim {2 * half} exceeds the head dim {min(dims)}")
+    axes, at = 1, (0, 0, 1, 0, 0)
+    if positions is not None:
+        if positions.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"positions must be int32 or int64; got {positions.dtype}")
+        if positions.device != device:
+            raise ValueError(f"positions is on {positions.device}; expected {device}")
+        shape = positions.shape
+        if len(shape) not in (1, 2) or shape[-1] != tokens or (len(shape) == 2 and not 1 <= shape[0] <= 4):
+            raise ValueError(f"positions {tuple(shape)} must be [{tokens}] or [axes, {tokens}] with 1 to 4 axes")
+        axes = shape[0] if len(shape) == 2 else 1
+        at = (positions.data_ptr(), _lib.I64 if positions.dtype == torch.int64 else _lib.I32, axes,
+              positions.stride(0) if len(shape) == 2 else 0, positions.stride(-1))
+    if pair_axes is not None and type(pair_axes) is not tuple:
+        if torch.is_tensor(pair_axes):
+            raise TypeError("pair_axes is a sequence of ints on the host")
+        pair_axes = tuple(pair_axes)
+    return (cos.data_ptr(), sin.data_ptr(), _lib.DTYPE_CODE[cos.dtype], int(bool(interleaved)), half, rows,
+            *cos.stride(), *sin.stride(), *at, *_pair_axis_words(pair_axes, half, axes))
+
+
+def _check_rows(**rows):
+    """Packed rows [tokens, heads, dim] on one GPU, of one input type and token count."""
+    first = None
+    for name, x in rows.items():
+        if x is None:
+            continue
+        if not on_gpu(x):
+            raise ValueError(f"{name} is on {x.device}; cache operations run on a ROCm GPU")
+        if x.ndim != 3 or not 1 <= x.shape[2] <= 512 or x.shape[1] < 1:
+            raise ValueError(f"{name} {tuple(x.shape)} must be [tokens, heads, dim] with dim in 1..512")
+        if x.dtype not in _INPUT_TYPES:
+            raise TypeError(f"{name} is {x.dtype}; rows are float16, bfloat16 or float32")
+        if first is None:
+            first = x
+        elif x.shape[0] != first.shape[0] or x.device != first.device:
+            raise ValueError(f"{name} {tuple(x.shape)} on {x.device} does not go with {tuple(first.shape)} on {first.device}")
+        elif x.dtype != first.dtype:
+            raise TypeError(f"{name} is {x.dtype}; the rows of one call share one type, here {first.dtype}")
+    return first
+
+
+_NO_ROWS = (0,) * 7
+
+
+def _rows(x, out):
+    """The fa_rows fields of rows x written to contiguous `out`."""
+    return x.data_ptr(), out.data_ptr(), x.shape[1], x.shape[2], *x.stride()
+
+
+def rotary_embedding(q, k, cos, sin, positions, *, pair_axes=None, interleaved=True):
+    """q [T, Hq, D] and k [T, Hk, D] (None: q alone) turned, as fresh tensors."""
+    reject_training(tensors=(q, k, cos, sin))
+    _check_rows(q=q, k=k)
+    tokens, device = q.shape[0], q.device
+    if positions is None:
+        raise ValueError("rotary_embedding needs the rows' positions")
+    rot = _rotation(cos, sin, positions, pair_axes, interleaved, tokens,
+                    [q.shape[2]] if k is None else [q.shape[2], k.shape[2]], device)
+    out_q = torch.empty(q.shape, dtype=q.dtype, device=device)
+    out_k = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=device)
+    if tokens:
+        a = _lib.pack_rotary_rows(*_rows(q, out_q), *(_NO_ROWS if k is None else _rows(k, out_k)), tokens,
+                                  _lib.DTYPE_CODE[q.dtype], 0, *rot)
+        _lib.call("fa_rotary_rows", a, device)
+    return out_q, out_k
+
+
+def append_paged_kvcache(k, v, k_cache, v_cache, cu_seqlens_q, seqused_k, block_table, *, q=None, cos=None, sin=None,
+                         positions=None, pair_axes=None, interleaved=True, k_scale=None, v_scale=None):
+    """The rows of each request, its last seqused_k[b] positions, into its pages (see the package's function)."""
+    reject_training(tensors=(k, v, k_cache, v_cache, q, cos, sin))
+    _check_rows(k=k, v=v, q=q)
+    tokens, heads = k.shape[:2]
+    device = k.device
+    if v.shape[1] != heads:
+        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must have the same heads")
+    for name, x, cache in (("k_cache", k, k_cache), ("v_cache", v, v_cache)):
+        if cache.device != device:
+            raise ValueError(f"{name} is on {cache.device}; expected {device}")
+        _check_cache_shape(x, cache, 1)
+        if cache.dtype != k.dtype and cache.dtype != torch.float8_e4m3fn:
+            raise TypeError(f"a {cache.dtype} cache cannot take {k.dtype} rows (use the same dtype or float8_e4m3fn)")
+    pages, size = k_cache.shape[:2]
+    if v_cache.shape[:2] != k_cache.shape[:2] or v_cache.dtype != k_cache.dtype or size < 1:
+        raise ValueError("the K and V caches must have the same pages, page size and type")
+    batch = seqused_k.shape[0] if torch.is_tensor(seqused_k) and seqused_k.ndim == 1 else -1
+    for t, name, shape in ((cu_seqlens_q, "cu_seqlens_q", (batch + 1,)), (seqused_k, "seqused_k", (batch,)),
+                           (block_table, "block_table", (batch, None))):
+        if not torch.is_tensor(t) or batch < 0:
+            raise ValueError("cu_seqlens_q, seqused_k and block_table are int32 tensors [B + 1], [B] and [B, pages]")
+        Want(name, shape, (torch.int32,)).check(t, device)
+    if is_block_scale(k_scale) != is_block_scale(v_scale):
+        raise ValueError("k_scale and v_scale are both scales per block (float8_e8m0fnu) or neither")
+    keep, block, block_ptrs, block_strides, head_scale = [], 0, (0, 0), (0,) * 6, ((0, 0), (0, 0))
+    if is_block_scale(k_scale):
+        block = block_of(k_cache, k_scale, "k_scale")
+        if block_of(v_cache, v_scale, "v_scale") != block:
+            raise ValueError("the K and V scales must have the same tokens per block")
+        block_ptrs, block_strides = (k_scale.data_ptr(), v_scale.data_ptr()), (*k_scale.stride(), *v_scale.stride())
+    elif k_cache.dtype == torch.float8_e4m3fn:
+        keep = [_per_head_scale(s, heads, device) for s in (k_scale, v_scale)]
+        head_scale = [(s.data_ptr(), stride) for s, stride in keep]
+    if (cos is None) != (sin is None):
+        raise ValueError("rotary_cos and rotary_sin come together")
+    if cos is None:
+        if q is not None or positions is not None or pair_axes is not None:
+            raise ValueError("q, positions and pair_axes go with rotary_cos and rotary_sin")
+        rot = _NO_ROTATION
+    else:
+        rot = _rotation(cos, sin, positions, pair_axes, interleaved, tokens,
+                        [k.shape[2]] if q is None else [k.shape[2], q.shape[2]], device)
+    out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=device)
+    if tokens:
+        code = _lib.DTYPE_CODE
+        descs = []
+        for x, cache, (scale, stride) in ((k, k_cache, head_scale[0]), (v, v_cache, head_scale[1])):
+            descs += (x.data_ptr(), cache.data_ptr(), scale, code[x.dtype], code[cache.dtype], heads, x.shape[2],
+                      *x.stride(), *cache.stride(), stride)
+        a = _lib.pack_append(*descs, *block_ptrs, *block_strides, block, *(_NO_ROWS if q is None else _rows(q, out)), *rot,
+                             cu_seqlens_q.data_ptr(), cu_seqlens_q.stride(0), seqused_k.data_ptr(), seqused_k.stride(0),
+                             block_table.data_ptr(), *block_table.stride(), tokens, batch, size, pages,
+                             block_table.shape[1])
+        _lib.call("fa_paged_append", a, device)
+    return out

@@ -96,15 +96,19 @@ class AttnArgs(ctypes.Structure):
 
 
 def _packer(struct_type):
-    """A struct.Struct of the C layout: one pack() sets every field (arrays
-    flattened, pointers as ints), where ctypes sets them one by one (~10 us
-    for an attention call's 90 values, 3 us packed)."""
-    codes = {_p: "P", _i32: "i", _i64: "q", _f32: "f"}
-    fmt = ""
-    for _, t in struct_type._fields_:
-        n = getattr(t, "_length_", 1)
-        fmt += codes[getattr(t, "_type_", t) if n > 1 else t] * n
-    s = struct.Struct("@" + fmt)
+    """A struct.Struct of the C layout: one pack() sets every field (arrays and
+    inner structures flattened, pointers as ints), where ctypes sets them one by
+    one (~10 us for an attention call's 90 values, 3 us packed)."""
+    codes = {_p: "P", _i32: "i", _i64: "q", _f32: "f", ctypes.c_uint64: "Q"}
+
+    def layout(t):
+        if t in codes:
+            return codes[t]
+        if issubclass(t, ctypes.Array):
+            return layout(t._type_) * t._length_
+        return "".join(layout(field) for _, field in t._fields_)
+
+    s = struct.Struct("@" + layout(struct_type))
     assert s.size == ctypes.sizeof(struct_type)
     return s
 
@@ -114,10 +118,43 @@ _attn_packer = _packer(AttnArgs)
 
 def pack_attn(*values):
     """An AttnArgs from its fields' values in order, arrays flattened."""
+    return _pack(AttnArgs, _attn_packer, "attention", values)
+
+
+def _pack(struct_type, packer, what, values):
     try:
-        return AttnArgs.from_buffer_copy(_attn_packer.pack(*values))
+        return struct_type.from_buffer_copy(packer.pack(*values))
     except struct.error as e:
-        raise TypeError(f"attention sizes and scalars: {e}") from e
+        raise TypeError(f"{what} sizes and scalars: {e}") from e
+
+
+class BlockAttnArgs(ctypes.Structure):
+    _fields_ = [("size", _i64), ("attn", AttnArgs), ("k_scale", _p), ("v_scale", _p),
+                ("k_scale_stride", _arr(_i64, 3)), ("v_scale_stride", _arr(_i64, 3)), ("block", _i64)]
+
+
+class Rotation(ctypes.Structure):
+    _fields_ = [("cos_table", _p), ("sin_table", _p), ("trig_dtype", _i32), ("interleaved", _i32),
+                ("half_rot", _i64), ("table_rows", _i64), ("cos_stride", _arr(_i64, 2)), ("sin_stride", _arr(_i64, 2)),
+                ("positions", _p), ("position_dtype", _i32), ("axes", _i32), ("position_stride", _arr(_i64, 2)),
+                ("pair_axis", _arr(ctypes.c_uint64, 8))]
+
+
+class Rows(ctypes.Structure):
+    _fields_ = [("x", _p), ("out", _p), ("heads", _i64), ("dim", _i64), ("x_stride", _arr(_i64, 3))]
+
+
+class RotaryRowsArgs(ctypes.Structure):
+    _fields_ = [("size", _i64), ("rows", _arr(Rows, 2)), ("tokens", _i64), ("dtype", _i32), ("_pad0", _i32),
+                ("rot", Rotation)]
+
+
+class PagedAppendArgs(ctypes.Structure):
+    _fields_ = [("size", _i64), ("kv", _arr(StoreDesc, 2)), ("block_scale", _arr(_p, 2)),
+                ("block_stride", _arr(_i64, 6)), ("block", _i64), ("q", Rows), ("rot", Rotation),
+                ("cu_seqlens_q", _p), ("cu_q_stride", _i64), ("seqused_k", _p), ("used_k_stride", _i64),
+                ("block_table", _p), ("bt_stride", _arr(_i64, 2)),
+                ("tokens", _i64), ("batch", _i64), ("page_size", _i64), ("num_pages", _i64), ("table_cols", _i64)]
 
 
 class MergePairArgs(ctypes.Structure):
@@ -137,6 +174,19 @@ class MergePartialsArgs(ctypes.Structure):
                 ("out_stride", _arr(_i64, 3)), ("lse_stride", _arr(_i64, 2))]
 
 
+_rotary_packer, _append_packer = _packer(RotaryRowsArgs), _packer(PagedAppendArgs)
+
+
+def pack_rotary_rows(*values):
+    """A RotaryRowsArgs from its fields' values after `size`."""
+    return _pack(RotaryRowsArgs, _rotary_packer, "rotary", (_rotary_packer.size, *values))
+
+
+def pack_append(*values):
+    """A PagedAppendArgs from its fields' values after `size`."""
+    return _pack(PagedAppendArgs, _append_packer, "append", (_append_packer.size, *values))
+
+
 STRUCTS = (StoreArgs, AppendArgs, RotaryArgs, AttnArgs, MergePairArgs, MergePartialsArgs)
 
 # Entry points declared in include/fa_gfx950.h: name -> (argument struct or None, restype).
@@ -148,6 +198,9 @@ ENTRY_POINTS = {
     "fa_append_kvcache": (AppendArgs, ctypes.c_int),
     "fa_rotary": (RotaryArgs, ctypes.c_int),
     "fa_rotary_append": (StepArgs, ctypes.c_int),
+    "fa_rotary_rows": (RotaryRowsArgs, ctypes.c_int),
+    "fa_paged_append": (PagedAppendArgs, ctypes.c_int),
+    "fa_block_attn_fwd": (BlockAttnArgs, ctypes.c_int),
     "fa_decode_supported": (AttnArgs, ctypes.c_int),
     "fa_decode_fwd": (AttnArgs, ctypes.c_int),
     "fa_decode_fwd_noalloc": (AttnArgs, ctypes.c_int),
@@ -213,6 +266,9 @@ def _function(name):
 
 
 def call(name, args, device):
+    if device.index is not None and device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):   # a launch goes to the current device's stream handles
+            return call(name, args, device)
     rc = _function(name)(ctypes.byref(args), stream_of(device))
     if rc != 0:
         raise RuntimeError(f"{name} failed ({rc}): {load().fa_last_error().decode()}")

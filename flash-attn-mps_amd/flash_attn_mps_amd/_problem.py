@@ -171,6 +171,11 @@ class Problem:
         return self.k.ndim == 4
 
     @property
+    def block_scaled(self):
+        """Whether K/V are a block-scaled cache: E8M0 scales in place of descales."""
+        return self.k_descale is not None and self.k_descale.dtype == torch.float8_e8m0fnu
+
+    @property
     def output_dtype(self):
         """FP8 queries produce fp16 (flash_attn_mps/_attention.py:120); others keep their type."""
         return torch.float16 if self.q.dtype == torch.float8_e4m3fn else self.q.dtype
@@ -233,8 +238,11 @@ class Problem:
         if torch.is_tensor(self.causal):
             _check(self.causal, "dynamic causal flags", (b,), (torch.bool,), device)
         _check(self.q_descale, "q_descale", (b, hk), f32, device)
-        _check(self.k_descale, "k_descale", (b, hk), f32, device)
-        _check(self.v_descale, "v_descale", (b, hk), f32, device)
+        if self.block_scaled:
+            self._validate_block_scales()
+        else:
+            _check(self.k_descale, "k_descale", (b, hk), f32, device)
+            _check(self.v_descale, "v_descale", (b, hk), f32, device)
         if self.alibi is not None:
             Want("alibi_slopes", {(hq,), (b, hq)}, f32).check(self.alibi, device)
         _check(self.sinks, "s_aux", (hq,), (), device)
@@ -260,3 +268,18 @@ class Problem:
             # Single-query rows: at most one per request.
             raise ValueError(f"{self.tokens} query rows for {b} requests with max_seqlen_q=1")
         return self
+
+    def _validate_block_scales(self):
+        """k_descale and v_descale as E8M0 scales [pages, page_size / block, Hkv] of a paged E4M3 cache."""
+        k, v = self.k, self.v
+        if not (self.paged and k.dtype == v.dtype == torch.float8_e4m3fn):
+            raise TypeError("float8_e8m0fnu descales (a scale per block) go with a paged float8_e4m3fn cache")
+        if self.leftpad is not None or self.used_k is None:
+            raise ValueError("a block-scaled cache takes lengths (seqused_k) and no left padding")
+        shape = (k.shape[0], None, k.shape[2])
+        _check(self.k_descale, "k_descale", shape, (torch.float8_e8m0fnu,), self.device)
+        _check(self.v_descale, "v_descale", shape, (torch.float8_e8m0fnu,), self.device)
+        if self.v_descale is None or self.v_descale.shape != self.k_descale.shape:
+            raise ValueError("block scales of K and V come together, in one shape")
+        if not self.k_descale.shape[1] or k.shape[1] % self.k_descale.shape[1]:
+            raise ValueError(f"{self.k_descale.shape[1]} scales a page do not divide pages of {k.shape[1]} tokens")

@@ -2,7 +2,8 @@
 
 Counterpart of flash_attn_mps/vllm.py (vLLM 0.29.0's argument order):
 per-request ("dynamic") causality, the multimodal-prefix and rolling-window
-masks, FP8 descales ``[B, Hkv]`` (broadcast views allowed), attention sinks
+masks, FP8 descales ``[B, Hkv]`` (broadcast views allowed) or a scale per block
+of a paged cache, attention sinks
 (``s_aux``), caller-owned ``out``, split-KV and LSE merging for cascade /
 decode-context-parallel attention.  It registers no vLLM platform and moves
 no data between GPUs: ``merge_attn_states`` is the local combine step of
@@ -70,6 +71,10 @@ def flash_attn_varlen_func(
     ``causal`` per request.  ``num_splits=1`` (or ``deterministic``) gives
     every query row a fixed reduction order whatever else is in the batch.
     Paged K/V requires ``seqused_k``.
+
+    ``k_descale`` / ``v_descale`` are float32 [B, Hkv], or, for a paged E4M3 cache as
+    ``append_paged_kvcache`` fills it, float8_e8m0fnu [pages, page_size / block, Hkv]:
+    a power of two per block of tokens and head, in place of descales.
     """
     reject_training(dropout_p, return_attn_probs, (q, k, v))
     if fa_version not in (2, 3, 4):

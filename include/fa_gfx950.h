@@ -139,6 +139,66 @@ typedef struct fa_step_args {
   int32_t* lengths_out;        /* [batch]: lengths + new_tokens - leftpad; NULL: not written */
 } fa_step_args;
 
+/* Rotary embedding of packed rows: pair i of a head (dims 2 i, 2 i + 1
+ * interleaved, else i, i + half_rot) turns by the angle of row
+ * positions[axis of i][token] of the cos/sin tables; a position without a row
+ * gives NaN. */
+typedef struct fa_rotation {
+  const void* cos_table; const void* sin_table;   /* [table_rows, half_rot] of trig_dtype; NULL: no rotation */
+  int32_t trig_dtype;          /* FA_F16 / FA_BF16 / FA_F32 */
+  int32_t interleaved;
+  int64_t half_rot, table_rows;   /* half_rot <= 256 */
+  int64_t cos_stride[2], sin_stride[2];
+  const void* positions;       /* [axes, tokens]; NULL (append only): the rows' cache positions */
+  int32_t position_dtype;      /* FA_I32 / FA_I64 */
+  int32_t axes;                /* 1..4 */
+  int64_t position_stride[2];
+  uint64_t pair_axis[8];       /* two bits per pair, 32 pairs a word */
+} fa_rotation;
+
+/* Rows [tokens, heads, dim] with any strides -> contiguous rows. */
+typedef struct fa_rows {
+  const void* x; void* out;
+  int64_t heads, dim;
+  int64_t x_stride[3];
+} fa_rows;
+
+/* Rotary embedding of up to two sets of rows (rows[1].x NULL: one). */
+typedef struct fa_rotary_rows_args {
+  int64_t size;                /* sizeof(fa_rotary_rows_args) */
+  fa_rows rows[2];
+  int64_t tokens;
+  int32_t dtype;               /* FA_F16 / FA_BF16 / FA_F32 */
+  int32_t _pad0;
+  fa_rotation rot;
+} fa_rotary_rows_args;
+
+/* Append of packed rows to a paged cache, K rotated on the way, and the
+ * rotation of Q.  Request b owns rows cu_seqlens_q[b] .. cu_seqlens_q[b + 1],
+ * its last positions: row j of n lies at seqused_k[b] - n + j.  A position or
+ * page outside the table or the cache is skipped; rows in no request are not
+ * written, and their q is copied unless positions are given.  K rounds once,
+ * from the fp32 rotation to the cache's type.
+ *
+ * block > 0: a block-scaled cache (fa_block_attn_args).  A block that gets rows
+ * takes the smallest power of two >= 2^-100 under which its largest finite new
+ * magnitude is at most 448; if it holds earlier rows of its request, the
+ * larger of that and its old scale, under which those rows are coded again.
+ * Infinities saturate, NaN is kept. */
+typedef struct fa_paged_append_args {
+  int64_t size;                /* sizeof(fa_paged_append_args) */
+  fa_store_desc kv[2];         /* K and V, one head count; scale: E4M3 caches without blocks */
+  uint8_t* block_scale[2];     /* E8M0 [pages, page_size / block, heads] */
+  int64_t block_stride[2][3];
+  int64_t block;               /* tokens per scale, dividing page_size; 0: none */
+  fa_rows q;                   /* q.x NULL: none */
+  fa_rotation rot;
+  const int32_t* cu_seqlens_q; int64_t cu_q_stride;
+  const int32_t* seqused_k;    int64_t used_k_stride;
+  const int32_t* block_table;  int64_t bt_stride[2];
+  int64_t tokens, batch, page_size, num_pages, table_cols;
+} fa_paged_append_args;
+
 /* ------------------------------------------------------------- attention */
 
 /* Attention over packed [T, Hkv, D] or paged [pages, P, Hkv, D] K/V.  Output
@@ -198,6 +258,20 @@ typedef struct fa_attn_args {
  * row untouched (a caller routes those to fa_decode_fwd in the same batch). */
 #define FA_FLAG_SKIP_SINGLE_QUERY 1
 
+/* Attention over a block-scaled cache: attn.k / attn.v are paged E4M3 codes
+ * [pages, P, Hkv, D], and rows j * block .. of a page carry one power of two per
+ * head, the E8M0 byte e at k_scale[page * stride[0] + j * stride[1] + head *
+ * stride[2]] (j < P / block, `block` dividing P): a value is code * 2^(e - 127),
+ * NaN with e = 255.  attn.k_descale / v_descale are NULL, attn.q is any input type.  No counterpart in the
+ * reference, whose FP8 caches have one scale per request and head. */
+typedef struct fa_block_attn_args {
+  int64_t size;                /* sizeof(fa_block_attn_args) */
+  fa_attn_args attn;
+  const uint8_t* k_scale; const uint8_t* v_scale;
+  int64_t k_scale_stride[3], v_scale_stride[3];
+  int64_t block;               /* tokens per scale */
+} fa_block_attn_args;
+
 /* Two-state merge (out may alias a or b, out_lse may alias a_lse). */
 typedef struct fa_merge_pair_args {
   void* out; const void* a; const void* b;
@@ -231,6 +305,9 @@ int fa_store_kvcache(const fa_store_args* args, void* stream);
 int fa_append_kvcache(const fa_append_args* args, void* stream);
 int fa_rotary(const fa_rotary_args* args, void* stream);
 int fa_rotary_append(const fa_step_args* args, void* stream);
+
+int fa_rotary_rows(const fa_rotary_rows_args* args, void* stream);
+int fa_paged_append(const fa_paged_append_args* args, void* stream);
 
 /* Split-KV decode.  With max_seqlen_q <= 1: one query row per request (rows
  * with cu_seqlens_q difference 1; others are skipped).  With max_seqlen_q = R
@@ -284,6 +361,9 @@ int fa_prefill_fwd(const fa_attn_args* args, void* stream);
  * dtypes.  num_splits > 1 requires partial_out [S, T, Hq, Dv] and
  * partial_lse [S, Hq, T] and merges into out/lse. */
 int fa_attn_fwd(const fa_attn_args* args, void* stream);
+
+/* fa_attn_fwd over a block-scaled cache. */
+int fa_block_attn_fwd(const fa_block_attn_args* args, void* stream);
 
 int fa_merge_pair(const fa_merge_pair_args* args, void* stream);
 int fa_merge_partials(const fa_merge_partials_args* args, void* stream);
