@@ -101,8 +101,10 @@ inline A fa_bounded(const A& args) {
 // Host-side argument checks shared by fa_attn_fwd / fa_decode_fwd / fa_prefill_fwd.
 int fa_validate_attn(const fa_attn_args* a, const char* who);
 
-// The checks of a block-scaled call, and its kernel arguments in `out` (window
-// bounds as fa_bounded gives them).
+// The kernel arguments of a block-scaled call in `out` (window bounds as
+// fa_bounded gives them); false where the structure or its block size are not
+// those of one.  fa_validate_block also checks the attention's arguments.
+bool fa_block_arguments(const fa_block_attn_args* args, fa_block_attn* out);
 int fa_validate_block(const fa_block_attn_args* args, fa_block_attn* out, const char* who);
 
 // fa_merge_partials for the splits of one call: a NaN LSE makes the row NaN,

@@ -8,6 +8,16 @@
 
 #include "attn_common.h"
 
+// The arguments of a kernel whose first parameter they are, through an address
+// that the compiler cannot see into: a rarely taken route then loads what it
+// needs when it runs, where its uses of the parameter itself would keep two
+// hundred scalars for the whole kernel.
+FA_DEV const fa_block_attn& block_arguments() {
+  auto p = (const fa_block_attn*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *p;
+}
+
 // q(d): the query's element d.  emit(d, x): output element d, normalised.  The
 // row sees keys of [begin, end) that key_allowed lets through; the sink joins
 // split 0.  Returns the LSE: -inf without a key, NaN where the sum is.

@@ -44,6 +44,7 @@
 #ifndef FA_DECODE_GQA_H
 #define FA_DECODE_GQA_H
 
+#include "block_row.h"
 #include "decode_kernel.h"
 #include "prefill_kernel.h"
 
@@ -187,8 +188,15 @@ FA_DEV void e4m3_row(const fa_attn_args& a, int64_t b, const RequestInfo& r, int
 // two fp16 terms, which drop what lies 2^25 below the running maximum: 32 x
 // 8192 keys 32/8 d128 105.8 -> 110.4 us a call, 64 x 16384 64/8 366.6 -> 370.5.
 // Two waves per SIMD are asked for, which the softcap variants would lose.
-template <typename T, int D, bool CAP, typename KT = T, int PACK = 1, bool QF8 = false>
-__global__ __launch_bounds__(GQA_THREADS, QF8 ? 2 : 1) void decode_gqa_kernel(const fa_attn_args a, const int span) {
+// BLOCK: a block-scaled cache (E4M3 codes, blocks of a multiple of 16 keys): each
+// 16-key group has one K and one V scale per KV head, kept beside its page on a
+// lane and handed over by v_readlane.  K's multiplies the scores in fp32, V's
+// enters the widening conversion, which takes a power of two for nothing; so the
+// loop has the E4M3 kernel's arithmetic.  A column whose sum is not finite runs
+// again by block_row, which reads only what a row sees.
+template <typename T, int D, bool CAP, typename KT = T, int PACK = 1, bool QF8 = false, bool BLOCK = false>
+__global__ __launch_bounds__(GQA_THREADS, QF8 || BLOCK ? 2 : 1) void decode_gqa_kernel(const typename AttnArgsOf<BLOCK>::type a,
+                                                                             const int span) {
   static_assert(D == 64 || D == 128 || D == 256, "rows of 64, 128 or 256 elements");
   static_assert((PACK == 1 && D <= 128) || (PACK == 2 && (D == 128 || (D == 256 && KT::id == FA_E4M3))),
                 "paired heads: 64-dim heads, or 128-dim E4M3 heads");
@@ -206,6 +214,7 @@ __global__ __launch_bounds__(GQA_THREADS, QF8 ? 2 : 1) void decode_gqa_kernel(co
   constexpr bool RING2 = NSLOT == 4;      // slots hold two stages (E4M3, unpaired)
   static_assert(!QF8 || (FP8 && T::id == FA_BF16), "E4M3 queries: E4M3 K/V, bf16 products");
   constexpr int PT = QF8 ? 3 : 1;         // 16-bit terms of a probability
+  static_assert(!BLOCK || (FP8 && !QF8), "block scales: E4M3 K/V, 16-bit queries");
 
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hh = lane >> 5;
@@ -380,6 +389,29 @@ __global__ __launch_bounds__(GQA_THREADS, QF8 ? 2 : 1) void decode_gqa_kernel(co
   // per 32 of its stages.
   int chunk = -1;
   uint32_t pages = 0;
+  // BLOCK: the scale bytes of lane l's group, K of each part, then V (bytes 2 and
+  // 3), for even and odd chunks: the DMA may be a chunk ahead of the arithmetic.
+  // The first chunk's are loaded behind the first DMAs, which they need not wait
+  // for; later ones with their pages.
+  uint32_t scales_even = 0, scales_odd = 0;
+  auto load_scales = [&](int ch) {
+    if constexpr (BLOCK) {
+      const int jj = 64 * ch + lane, pos = group_pos(jj);
+      uint32_t w = 0;
+      if (jj < ngroups && pos + 16 > pos_lo && pos < pos_end) {
+        const int row = pos % P;
+#pragma unroll
+        for (int u = 0; u < PACK; ++u)
+          w |= scale_byte(a, 0, pages, row, PACK * kh + u) << (8 * u) |
+               scale_byte(a, 1, pages, row, PACK * kh + u) << (16 + 8 * u);
+      }
+      if (ch & 1) scales_odd = w;
+      else scales_even = w;
+    }
+  };
+  auto scales_of_group = [&](int j) {
+    return (uint32_t)__builtin_amdgcn_readlane((int)((j >> 6) & 1 ? scales_odd : scales_even), j & 63);
+  };
   auto page_of_group = [&](int j) {
     if ((j >> 6) != chunk) {
       chunk = j >> 6;
@@ -387,6 +419,10 @@ __global__ __launch_bounds__(GQA_THREADS, QF8 ? 2 : 1) void decode_gqa_kernel(co
       const bool need = jj < ngroups && pos + 16 > pos_lo && pos < pos_end;
       pages = need ? (uint32_t)trow[(int64_t)(pos / P) * a.bt_stride[1]] : 0u;
       wait_dma_older_than<0>();
+      if (BLOCK && chunk > 0) {
+        load_scales(chunk);
+        wait_dma_older_than<0>();
+      }
     }
     return (uint32_t)__builtin_amdgcn_readlane((int)pages, j & 63);
   };
@@ -527,6 +563,16 @@ __global__ __launch_bounds__(GQA_THREADS, QF8 ? 2 : 1) void decode_gqa_kernel(co
     } else {
       if (more) dma_k_stage(i + 1);
     }
+    // BLOCK: the scores' scale is that of the key's group, s[8 c ..] of group c.
+    float block_k[2] = {1.0f, 1.0f};
+    uint32_t group_scales[2] = {0u, 0u};
+    if constexpr (BLOCK) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        group_scales[c] = scales_of_group(2 * i + c);
+        block_k[c] = e8m0_to_f32((group_scales[c] >> (8 * cpart)) & 255u);
+      }
+    }
     // s[e] = score of storage position st_pos(i) + 16 (e >> 3) + 8 hh + (e & 7).
     const int p0 = st_pos(i) + 8 * hh;
     if constexpr (CAP && QF8) {
@@ -544,6 +590,7 @@ __global__ __launch_bounds__(GQA_THREADS, QF8 ? 2 : 1) void decode_gqa_kernel(co
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       float v = s[e];
+      if constexpr (BLOCK) v *= block_k[e >> 3];
       if constexpr (CAP && !QF8) v = cap_out * (1.0f - 2.0f * __builtin_amdgcn_rcpf(fast_exp2(cap_in * v) + 1.0f));
       else if constexpr (!CAP) v *= c_scale;
       const int pos = p0 + 16 * (e >> 3) + (e & 7);
@@ -613,8 +660,9 @@ __global__ __launch_bounds__(GQA_THREADS, QF8 ? 2 : 1) void decode_gqa_kernel(co
         u32x4 av;
         if constexpr (FP8) {
           const u32x2 w = lds_read_tr8(vb, vrd8[db]);
-          av = u32x4{widen_fp8_pair<T, false>(w[0]), widen_fp8_pair<T, true>(w[0]), widen_fp8_pair<T, false>(w[1]),
-                     widen_fp8_pair<T, true>(w[1])};
+          const float vs = BLOCK ? e8m0_to_f32((group_scales[c] >> (16 + 8 * (db / DBH))) & 255u) : 1.0f;
+          av = u32x4{widen_fp8_pair<T, false>(w[0], vs), widen_fp8_pair<T, true>(w[0], vs),
+                     widen_fp8_pair<T, false>(w[1], vs), widen_fp8_pair<T, true>(w[1], vs)};
         } else {
           const int vrd = ((db & 1) ? vrd1 : vrd0) + (db >> 1) * KGROUP;
           const u32x2 lo = lds_read_tr(vb, vrd);
@@ -640,6 +688,10 @@ __global__ __launch_bounds__(GQA_THREADS, QF8 ? 2 : 1) void decode_gqa_kernel(co
     dma_k_stage(1);
     dma_v_stage(1);
   }
+  if (BLOCK && nst > 0) {
+    load_scales(0);
+    wait_dma_older_than<0>();
+  }
   for (int i = 0; i < nst; ++i) stage(i, i + 1 < nst);
 
   // ---- Combine the four waves: per head m (log2 units), l and O^T through
@@ -648,7 +700,7 @@ __global__ __launch_bounds__(GQA_THREADS, QF8 ? 2 : 1) void decode_gqa_kernel(co
   __syncthreads();
   float* const cm = (float*)smem;                      // [4][32]
   float* const cl = cm + 4 * GQA_HEADS;                // [4][32]
-  constexpr bool PROBE = QF8 && PACK > 1;   // [4]: whether a wave's sums are all finite
+  constexpr bool PROBE = (QF8 && PACK > 1) || BLOCK;   // [4]: whether a wave's sums are finite
   int* const finite = (int*)(cl + 4 * GQA_HEADS);
   // [4][32][DH + 4]: the 4-float pad puts the 32 head columns' 16-byte
   // stores of one instruction on distinct bank groups.
@@ -660,8 +712,9 @@ __global__ __launch_bounds__(GQA_THREADS, QF8 ? 2 : 1) void decode_gqa_kernel(co
     for (int db = 0; db < DBH; ++db)
 #pragma unroll
       for (int i = 0; i < 16; ++i) probe = fmaf(o[db][i], 0.0f, probe);
-    const bool ok = __all(probe == 0.0f);
-    if (lane == 0) finite[wave] = ok;
+    const uint64_t ok = __ballot(probe == 0.0f);
+    // BLOCK: the columns that are not (a column's sums lie on lanes l32 and l32 + 32).
+    if (lane == 0) finite[wave] = BLOCK ? (int)~((uint32_t)ok & (uint32_t)(ok >> 32)) : ok == ~0ull;
   }
   if (hh == 0) {
     cm[wave * GQA_HEADS + l32] = m_run;
@@ -675,7 +728,29 @@ __global__ __launch_bounds__(GQA_THREADS, QF8 ? 2 : 1) void decode_gqa_kernel(co
       *(float4*)(co + ((int64_t)wave * GQA_HEADS + l32) * CO_ROW + 32 * db + 8 * g + 4 * hh) =
           float4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
   __syncthreads();
-  if constexpr (PROBE) {
+  uint32_t bad = 0;   // BLOCK: columns that block_row writes
+  if constexpr (BLOCK) {
+    bad = (uint32_t)(finite[0] | finite[1] | finite[2] | finite[3]);
+    if (__builtin_expect(bad != 0, 0)) {
+      const fa_block_attn& ra = block_arguments();
+      for (int c = wave; c < nheads * ntok; c += 4) {
+        const int h = h0 + c / ntok, tt = c % ntok;
+        if (!(bad >> c & 1) || tt >= r.q_len) continue;
+        const int64_t tq = r.q_begin + tt, orow = ((b * ra.num_splits + split) * ntok + tt) * ra.heads_q + h;
+        const bool last = ra.num_splits == 1;
+        const float lse = block_row<DH / 64>(
+            ra, b, r, h / gr, h, split, tq, r.k_len - r.q_len + tt, begin, end, lane,
+            [&](int d) { return load_elem<T>(ra.q, tq * ra.q_stride[0] + (int64_t)h * ra.q_stride[1] + d); },
+            [&](int d, float x) {
+              if (last) store_any(ra.out, tq * ra.out_stride[0] + (int64_t)h * ra.out_stride[1] + d * ra.out_stride[2], ra.out_dtype, x);
+              else ra.partial_out[orow * DH + d] = x;
+            });
+        if (lane != 0) continue;
+        if (last) ra.lse[(int64_t)h * ra.lse_stride[0] + tq * ra.lse_stride[1]] = lse != lse ? -INFINITY : lse;
+        else ra.partial_lse[((b * ntok + tt) * ra.heads_q + h) * ra.num_splits + split] = lse;
+      }
+    }
+  } else if constexpr (PROBE) {
     if (__builtin_expect(!(finite[0] & finite[1] & finite[2] & finite[3]), 0)) {
       for (int c = wave; c < nheads; c += 4) {
         const int own = PACK * kh + part_of(c);
@@ -716,7 +791,7 @@ __global__ __launch_bounds__(GQA_THREADS, QF8 ? 2 : 1) void decode_gqa_kernel(co
   for (int idx = tid; idx < ncol * DH; idx += GQA_THREADS) {
     const int hc = idx / DH, d = idx - hc * DH;   // column hc: head h0 + hc / ntok, token hc % ntok
     const int th = (int)(((uint64_t)hc * ntok_inv) >> 32), tt = hc - th * ntok;
-    if (th >= nheads || tt >= r.q_len) continue;
+    if (th >= nheads || tt >= r.q_len || (BLOCK && bad >> hc & 1)) continue;
     float O = 0.0f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) O += co[((int64_t)w * GQA_HEADS + hc) * CO_ROW + d] * cm[w * GQA_HEADS + hc];

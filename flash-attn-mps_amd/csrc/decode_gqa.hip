@@ -26,11 +26,11 @@ bool chunks_aligned(const fa_attn_args& a, int kvb) {
   return true;
 }
 
-template <typename T, typename KT, int D, int PACK, bool QF8>
-GqaChoice choose(bool cap) {
-  GqaChoice c;
-  c.kern = cap ? fa_decode_gqa::decode_gqa_kernel<T, D, true, KT, PACK, QF8>
-               : fa_decode_gqa::decode_gqa_kernel<T, D, false, KT, PACK, QF8>;
+template <typename T, typename KT, int D, int PACK, bool QF8, bool BLOCK>
+GqaChoiceOf<typename AttnArgsOf<BLOCK>::type> choose(bool cap) {
+  GqaChoiceOf<typename AttnArgsOf<BLOCK>::type> c;
+  c.kern = cap ? fa_decode_gqa::decode_gqa_kernel<T, D, true, KT, PACK, QF8, BLOCK>
+               : fa_decode_gqa::decode_gqa_kernel<T, D, false, KT, PACK, QF8, BLOCK>;
   c.lds = fa_decode_gqa::gqa_lds_bytes<D, KT::id == FA_E4M3, PACK>();
   c.pack = PACK;
   return c;
@@ -61,50 +61,61 @@ bool packable(const fa_attn_args& a) {
          (fp8 || a.heads_k >= 8);
 }
 
-template <typename T, typename KT, bool QF8 = false>
-GqaChoice choose_dim(const fa_attn_args& a, bool cap) {
-  if (a.head_dim_qk == 64) return packable(a) ? choose<T, KT, 128, 2, QF8>(cap) : choose<T, KT, 64, 1, QF8>(cap);
+template <typename T, typename KT, bool QF8 = false, bool BLOCK = false>
+GqaChoiceOf<typename AttnArgsOf<BLOCK>::type> choose_dim(const fa_attn_args& a, bool cap) {
+  if (a.head_dim_qk == 64)
+    return packable(a) ? choose<T, KT, 128, 2, QF8, BLOCK>(cap) : choose<T, KT, 64, 1, QF8, BLOCK>(cap);
   if constexpr (KT::id == FA_E4M3) {
-    if (packable(a)) return choose<T, KT, 256, 2, QF8>(cap);
+    if (packable(a)) return choose<T, KT, 256, 2, QF8, BLOCK>(cap);
   }
-  return choose<T, KT, 128, 1, QF8>(cap);
+  return choose<T, KT, 128, 1, QF8, BLOCK>(cap);
 }
 
-}  // namespace
-
-GqaChoice pick_decode_gqa(const fa_attn_args& a) {
-  const GqaChoice none{nullptr, 0, 1};
-  if (a.heads_k <= 0 || a.heads_q % a.heads_k) return none;
-  // One query row per request: groups of DECODE_GQA_MIN_GROUP or more (the
-  // VALU kernel is faster below); 2..DECODE_GQA_MAX_ROWS rows: any group
-  // (nothing else runs a few rows per request as decode).
-  if (a.max_seqlen_q > DECODE_GQA_MAX_ROWS) return none;
-  if (a.max_seqlen_q <= 1 && a.heads_q / a.heads_k < DECODE_GQA_MIN_GROUP && !(a.head_dim_qk == 64 && packable(a)))
-    return none;
+// Types, head dims and layouts that the kernel takes, whatever the group.
+bool layout_ok(const fa_attn_args& a) {
+  if (a.heads_k <= 0 || a.heads_q % a.heads_k || a.max_seqlen_q > DECODE_GQA_MAX_ROWS) return false;
   // P.V runs on probabilities rounded to the query's type: fp32 outputs
   // (held to fp32 accuracy) take the VALU kernel, which keeps P in fp32.
   // E4M3 queries (P as three bf16 terms) write either 16-bit type; their
   // multi-row calls run as prefill.
   const bool fp8q = a.q_dtype == FA_E4M3;
   if (fp8q) {
-    if (a.max_seqlen_q > 1 || a.k_dtype != FA_E4M3 || (a.out_dtype != FA_F16 && a.out_dtype != FA_BF16)) return none;
+    if (a.max_seqlen_q > 1 || a.k_dtype != FA_E4M3 || (a.out_dtype != FA_F16 && a.out_dtype != FA_BF16)) return false;
   } else {
-    if (a.q_dtype != FA_BF16 && a.q_dtype != FA_F16) return none;
-    if (a.out_dtype != a.q_dtype) return none;
+    if (a.q_dtype != FA_BF16 && a.q_dtype != FA_F16) return false;
+    if (a.out_dtype != a.q_dtype) return false;
   }
-  if (a.k_dtype != a.v_dtype || (a.k_dtype != a.q_dtype && a.k_dtype != FA_E4M3)) return none;
-  if (a.head_dim_qk != a.head_dim_v || (a.head_dim_qk != 64 && a.head_dim_qk != 128)) return none;
-  if (a.alibi || a.mask_kind != 0) return none;
-  if (a.page_size && a.page_size % 16) return none;
+  if (a.k_dtype != a.v_dtype || (a.k_dtype != a.q_dtype && a.k_dtype != FA_E4M3)) return false;
+  if (a.head_dim_qk != a.head_dim_v || (a.head_dim_qk != 64 && a.head_dim_qk != 128)) return false;
+  if (a.alibi || a.mask_kind != 0) return false;
+  if (a.page_size && a.page_size % 16) return false;
   const int kvb = a.k_dtype == FA_E4M3 ? 1 : 2;
-  if (!chunks_aligned(a, kvb)) return none;
+  if (!chunks_aligned(a, kvb)) return false;
   // Row and page offsets are 32-bit byte counts in the kernel's addressing.
   for (int i = 0; i < 2; ++i)
-    if (a.k_stride[i] * kvb >= (1ll << 31) / 16 || a.v_stride[i] * kvb >= (1ll << 31) / 16) return none;
-  const bool cap = a.softcap > 0.0f, fp8 = a.k_dtype == FA_E4M3;
+    if (a.k_stride[i] * kvb >= (1ll << 31) / 16 || a.v_stride[i] * kvb >= (1ll << 31) / 16) return false;
+  return true;
+}
+
+}  // namespace
+
+GqaChoice pick_decode_gqa(const fa_attn_args& a) {
+  if (!layout_ok(a)) return GqaChoice{nullptr, 0, 1};
+  // One query row per request: groups of DECODE_GQA_MIN_GROUP or more (the
+  // VALU kernel is faster below); 2..DECODE_GQA_MAX_ROWS rows: any group
+  // (nothing else runs a few rows per request as decode).
+  if (a.max_seqlen_q <= 1 && a.heads_q / a.heads_k < DECODE_GQA_MIN_GROUP && !(a.head_dim_qk == 64 && packable(a)))
+    return GqaChoice{nullptr, 0, 1};
+  const bool cap = a.softcap > 0.0f, fp8 = a.k_dtype == FA_E4M3, fp8q = a.q_dtype == FA_E4M3;
   if (fp8q) return choose_dim<BF16T, E4M3T, true>(a, cap);
   if (a.q_dtype == FA_BF16) return fp8 ? choose_dim<BF16T, E4M3T>(a, cap) : choose_dim<BF16T, BF16T>(a, cap);
   return fp8 ? choose_dim<F16T, E4M3T>(a, cap) : choose_dim<F16T, F16T>(a, cap);
+}
+
+GqaChoiceOf<fa_block_attn> pick_decode_gqa(const fa_block_attn& a) {
+  if (!layout_ok(a) || a.k_dtype != FA_E4M3 || a.q_dtype == FA_E4M3 || a.block % 16) return {nullptr, 0, 1};
+  const bool cap = a.softcap > 0.0f;
+  return a.q_dtype == FA_BF16 ? choose_dim<BF16T, E4M3T, false, true>(a, cap) : choose_dim<F16T, E4M3T, false, true>(a, cap);
 }
 
 }  // namespace fa_decode

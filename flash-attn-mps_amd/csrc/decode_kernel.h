@@ -879,11 +879,15 @@ constexpr int DECODE_GQA_MIN_GROUP = 3;
 // Most query rows per request the matrix-core decode takes (its 32 columns
 // hold 32 / rows query heads).
 constexpr int DECODE_GQA_MAX_ROWS = 16;
-struct GqaChoice {
-  DecodeKernel kern;
+template <typename A>
+struct GqaChoiceOf {
+  void (*kern)(A, int);
   size_t lds;
-  int pack;   // KV heads per workgroup (2: neighbouring 64-dim or 128-dim E4M3 heads, PACK = 2)
+  int pack;   // KV heads per workgroup
 };
+using GqaChoice = GqaChoiceOf<fa_attn_args>;
 GqaChoice pick_decode_gqa(const fa_attn_args& a);
+// The same kernel over a block-scaled cache (16-bit queries, any group).
+GqaChoiceOf<fa_block_attn> pick_decode_gqa(const fa_block_attn& a);
 
 }  // namespace fa_decode

@@ -256,16 +256,10 @@ int64_t partial_rows(const fa_attn_args& a) {
   return a.batch * (a.max_seqlen_q > 1 ? a.max_seqlen_q : 1) * a.heads_q;
 }
 
-// Launch the decode kernel (and the merge when there are several splits) for
-// arguments that passed fa_validate_attn.
-int decode_launch(const fa_attn_args* a, void* stream, const char* who) {
-  int gt = 1;
-  const GqaChoice gqa = pick_decode_gqa(*a);
-  const DecodeKernel kern = gqa.kern ? gqa.kern : select_decode(*a, &gt);
-  if (!kern) {
-    fa_set_error("%s: unsupported dtype/head-dim/stride combination", who);
-    return FA_ERR_UNSUPPORTED;
-  }
+// Launch `kern`, over head_groups workgroups per (request, split), and the merge
+// when there are several splits, for arguments that passed their validation.
+template <typename A>
+int launch_splits(const A* a, void (*kern)(A, int), size_t lds, int64_t head_groups, void* stream, const char* who) {
   if (a->total_q == 0) return FA_OK;
   FA_REQUIRE(a->split_span >= 1 && a->num_splits >= 1, "%s: num_splits and split_span must be positive", who);
   // Keys past num_splits * split_span would be dropped without a trace.
@@ -274,18 +268,17 @@ int decode_launch(const fa_attn_args* a, void* stream, const char* who) {
              (long long)a->num_splits * a->split_span, (long long)decode_visible_max(*a));
   FA_REQUIRE(a->num_splits == 1 || (a->partial_out && a->partial_lse), "%s: splits need partial buffers", who);
   FA_REQUIRE(a->batch <= 65535, "%s: batch exceeds the grid limit", who);
-  const int64_t head_groups = decode_head_groups(*a, gt);
   FA_REQUIRE(a->num_splits <= 65535, "%s: too many splits", who);
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid((unsigned)head_groups, (unsigned)a->num_splits, (unsigned)a->batch);
-  if (gqa.kern) {
-    const hipError_t err = hipFuncSetAttribute((const void*)gqa.kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)gqa.lds);
+  if (lds) {
+    const hipError_t err = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (err != hipSuccess) {
-      fa_set_error("%s: cannot reserve %zu bytes of LDS: %s", who, gqa.lds, hipGetErrorString(err));
+      fa_set_error("%s: cannot reserve %zu bytes of LDS: %s", who, lds, hipGetErrorString(err));
       return FA_ERR_LAUNCH;
     }
   }
-  hipLaunchKernelGGL(kern, grid, dim3(DEC_THREADS), gqa.kern ? gqa.lds : 0, s, *a, (int)a->split_span);
+  hipLaunchKernelGGL(kern, grid, dim3(DEC_THREADS), lds, s, *a, (int)a->split_span);
   int rc = fa_check_launch(who);
   if (rc || a->num_splits == 1) return rc;
   const int64_t rows = partial_rows(*a);
@@ -295,6 +288,17 @@ int decode_launch(const fa_attn_args* a, void* stream, const char* who) {
                                                                       : decode_merge_kernel<4, 8>;
   hipLaunchKernelGGL(merge, dim3((unsigned)fa_ceil_div(rows, 4)), dim3(256), 0, s, *a, (int)a->split_span);
   return fa_check_launch(who);
+}
+
+int decode_launch(const fa_attn_args* a, void* stream, const char* who) {
+  int gt = 1;
+  const GqaChoice gqa = pick_decode_gqa(*a);
+  const DecodeKernel kern = gqa.kern ? gqa.kern : select_decode(*a, &gt);
+  if (!kern) {
+    fa_set_error("%s: unsupported dtype/head-dim/stride combination", who);
+    return FA_ERR_UNSUPPORTED;
+  }
+  return launch_splits(a, kern, gqa.kern ? gqa.lds : 0, a->total_q ? decode_head_groups(*a, gt) : 0, stream, who);
 }
 
 // Floats of the partial rows; the LSE rows start at the next 256-byte boundary.
@@ -369,6 +373,26 @@ extern "C" int fa_decode_fwd(const fa_attn_args* args, void* stream) {
   if (rc) return rc;
   const fa_attn_args a = fa_bounded(*args);
   return decode_launch(&a, stream, "fa_decode_fwd");
+}
+
+extern "C" int fa_block_decode_supported(const fa_block_attn_args* args) {
+  fa_block_attn a;
+  return fa_block_arguments(args, &a) && pick_decode_gqa(a).kern != nullptr;
+}
+
+extern "C" int fa_block_decode_fwd(const fa_block_attn_args* args, void* stream) {
+  const char* who = "fa_block_decode_fwd";
+  fa_block_attn a;
+  const int rc = fa_validate_block(args, &a, who);
+  if (rc) return rc;
+  const GqaChoiceOf<fa_block_attn> gqa = pick_decode_gqa(a);
+  if (!gqa.kern) {
+    fa_set_error("%s: unsupported dtype/head-dim/stride combination", who);
+    return FA_ERR_UNSUPPORTED;
+  }
+  const int64_t ntok = a.max_seqlen_q > 1 ? a.max_seqlen_q : 1;
+  const int64_t groups = a.heads_k / gqa.pack * fa_ceil_div(gqa.pack * (a.heads_q / a.heads_k), 32 / ntok);
+  return launch_splits(&a, gqa.kern, gqa.lds, groups, stream, who);
 }
 
 extern "C" int fa_decode_fwd_noalloc(const fa_attn_args* in, void* stream) {

@@ -176,17 +176,11 @@ int fa_validate_attn(const fa_attn_args* a, const char* who) {
   return FA_OK;
 }
 
-int fa_validate_block(const fa_block_attn_args* args, fa_block_attn* out, const char* who) {
-  FA_REQUIRE(args && args->size == (int64_t)sizeof(fa_block_attn_args), "%s: null or mismatched arguments", who);
+bool fa_block_arguments(const fa_block_attn_args* args, fa_block_attn* out) {
+  if (!args || args->size != (int64_t)sizeof(fa_block_attn_args)) return false;
   const fa_attn_args& a = args->attn;
-  const int rc = fa_validate_attn(&a, who);
-  if (rc) return rc;
-  FA_REQUIRE(a.k_dtype == FA_E4M3 && a.v_dtype == FA_E4M3 && a.page_size > 0 && a.seqused_k && !a.leftpad_k,
-             "%s: block scales go with a paged E4M3 cache", who);
-  FA_REQUIRE(!a.k_descale && !a.v_descale, "%s: block scales take the place of descales", who);
-  FA_REQUIRE(!a.k || (args->k_scale && args->v_scale), "%s: null scales", who);
-  FA_REQUIRE(args->block >= 1 && args->block <= a.page_size && a.page_size % args->block == 0 && a.page_size <= INT32_MAX,
-             "%s: a block must divide the page size", who);
+  if (a.k_dtype != FA_E4M3 || a.v_dtype != FA_E4M3 || a.page_size < 1 || a.page_size > INT32_MAX) return false;
+  if (args->block < 1 || args->block > a.page_size || a.page_size % args->block) return false;
   static_cast<fa_attn_args&>(*out) = fa_bounded(a);
   out->scale[0] = args->k_scale, out->scale[1] = args->v_scale;
   for (int i = 0; i < 3; ++i) {
@@ -194,6 +188,18 @@ int fa_validate_block(const fa_block_attn_args* args, fa_block_attn* out, const 
     out->scale_stride[1][i] = args->v_scale_stride[i];
   }
   out->block = (int32_t)args->block;
+  return true;
+}
+
+int fa_validate_block(const fa_block_attn_args* args, fa_block_attn* out, const char* who) {
+  FA_REQUIRE(args && args->size == (int64_t)sizeof(fa_block_attn_args), "%s: null or mismatched arguments", who);
+  const fa_attn_args& a = args->attn;
+  const int rc = fa_validate_attn(&a, who);
+  if (rc) return rc;
+  FA_REQUIRE(fa_block_arguments(args, out), "%s: block scales go with a paged E4M3 cache whose pages they divide", who);
+  FA_REQUIRE(a.seqused_k && !a.leftpad_k, "%s: a block-scaled cache takes lengths and no left padding", who);
+  FA_REQUIRE(!a.k_descale && !a.v_descale, "%s: block scales take the place of descales", who);
+  FA_REQUIRE(!a.k || (args->k_scale && args->v_scale), "%s: null scales", who);
   return FA_OK;
 }
 

@@ -102,19 +102,21 @@ template <> FA_DEV uint32_t pack2<F16T>(float lo, float hi) {
   return __builtin_bit_cast(uint32_t, v);
 }
 
-// Two E4M3 codes (bytes 2 HI .. 2 HI + 1 of w) -> two T values, exactly.
-template <typename T, bool HI> FA_DEV uint32_t widen_fp8_pair(uint32_t w);
-template <> FA_DEV uint32_t widen_fp8_pair<BF16T, false>(uint32_t w) {
-  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));
+// Two E4M3 codes (bytes 2 HI .. 2 HI + 1 of w) -> two T values times `scale`, a
+// power of two (the conversion takes its exponent): exact where T's range holds
+// them.
+template <typename T, bool HI> FA_DEV uint32_t widen_fp8_pair(uint32_t w, float scale = 1.0f);
+template <> FA_DEV uint32_t widen_fp8_pair<BF16T, false>(uint32_t w, float scale) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false));
 }
-template <> FA_DEV uint32_t widen_fp8_pair<BF16T, true>(uint32_t w) {
-  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true));
+template <> FA_DEV uint32_t widen_fp8_pair<BF16T, true>(uint32_t w, float scale) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true));
 }
-template <> FA_DEV uint32_t widen_fp8_pair<F16T, false>(uint32_t w) {
-  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false));
+template <> FA_DEV uint32_t widen_fp8_pair<F16T, false>(uint32_t w, float scale) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, false));
 }
-template <> FA_DEV uint32_t widen_fp8_pair<F16T, true>(uint32_t w) {
-  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true));
+template <> FA_DEV uint32_t widen_fp8_pair<F16T, true>(uint32_t w, float scale) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, true));
 }
 // w with its two 8-byte halves exchanged when `swap` (one select per dword).
 FA_DEV u32x4 halves_swapped_if(u32x4 w, int swap) {

@@ -142,7 +142,7 @@ def _fits_prefill(p, out):
     or E4M3 K/V with output in the query's type, or E4M3 queries over E4M3 K/V
     with fp16/bf16 output (S on the FP8 MFMA).  Deterministic calls qualify:
     prefill_splits keeps them, and num_splits=1, at one split."""
-    if p.splits not in (0, 1):
+    if p.splits not in (0, 1) or p.block_scaled:
         return False
     fp8 = torch.float8_e4m3fn
     if p.k.dtype != p.v.dtype:
@@ -318,7 +318,7 @@ def _mixed_batch(p, a, fixed_order=False):
     request only (the batch-invariant route)."""
     dec = _lib.AttnArgs.from_buffer_copy(a)
     dec.max_seqlen_q = 1   # the decode kernel takes the one-row requests only
-    if not _lib.supported("fa_decode_supported", dec):
+    if not supported(p, "fa_decode_supported", dec):
         return False
     from ._decode import decode_workgroups, split_plan
     groups = decode_workgroups(p, 1)
@@ -329,16 +329,16 @@ def _mixed_batch(p, a, fixed_order=False):
     a.flags |= _lib.FLAG_SKIP_SINGLE_QUERY
     kv_bytes = p.batch * p.visible_max * p.kv_heads * (p.dim_qk + p.dim_v) * p.k.element_size()
     if kv_bytes < _SIDE_STREAM_MIN_BYTES:
-        _lib.call("fa_prefill_fwd", a, p.device)
-        _lib.call("fa_decode_fwd", dec, p.device)
+        call(p, "fa_prefill_fwd", a)
+        call(p, "fa_decode_fwd", dec)
         return True
     main = torch.cuda.current_stream(p.device)
     side, fork, join = _side_stream(p.device)
     fork.record(main)
     side.wait_event(fork)
-    _lib.call("fa_prefill_fwd", a, p.device)
+    call(p, "fa_prefill_fwd", a)
     with torch.cuda.stream(side):
-        _lib.call("fa_decode_fwd", dec, p.device)
+        call(p, "fa_decode_fwd", dec)
     join.record(side)
     main.wait_event(join)
     return True
@@ -357,7 +357,7 @@ def _fixed_order_decode(p, out):
         return None
     lse = torch.empty((p.heads, p.tokens), device=p.device, dtype=torch.float32)
     a = build_args(p, out, lse)
-    if not (_lib.supported("fa_prefill_supported", a) and _lib.supported("fa_decode_supported", a)):
+    if not (supported(p, "fa_prefill_supported", a) and supported(p, "fa_decode_supported", a)):
         return None
     from ._decode import decode
     return decode(p, out, splits=1)
@@ -374,8 +374,6 @@ def solve(p):
         raise ValueError("nonempty queries need max_seqlen_q >= 1")
     if p.batch < 1:
         raise ValueError("cu_seqlens_q needs at least two offsets")
-    if p.block_scaled:
-        return _solve_generic(p, out)
     if p.max_q == 1 and not p.deterministic and p.mask is None:
         from ._decode import decode
         return decode(p, out)
@@ -392,7 +390,7 @@ def solve(p):
             return done
     lse = torch.empty((p.heads, p.tokens), device=p.device, dtype=torch.float32)
     a = build_args(p, out, lse)
-    if _fits_prefill(p, out) and _lib.supported("fa_prefill_supported", a):
+    if _fits_prefill(p, out) and supported(p, "fa_prefill_supported", a):
         # In a mixed chunked-prefill + decode batch the single-query requests
         # take the decode kernel: a 128-row MFMA query tile per head would be
         # almost empty for them.  Packed self-attention (queries and keys on
@@ -407,7 +405,7 @@ def solve(p):
             _partials(p, a, (splits, p.tokens, p.heads, p.dim_v), (splits, p.heads, p.tokens))
             a.num_splits, a.split_span = splits, prefill_split_span(p, splits)
         if not (mixed and _mixed_batch(p, a, fixed_order=p.deterministic)):
-            _lib.call("fa_prefill_fwd", a, p.device)
+            call(p, "fa_prefill_fwd", a)
         return out, lse
     per_row = p.deterministic or p.max_q == 1 or max(p.dim_qk, p.dim_v) > 256
     if p.deterministic:
@@ -417,13 +415,6 @@ def solve(p):
     if splits > 1:
         _partials(p, a, (splits, p.tokens, p.heads, p.dim_v), (splits, p.heads, p.tokens))
     a.num_splits = splits
-    _lib.call("fa_attn_fwd", a, p.device)
-    return out, lse
-
-
-def _solve_generic(p, out):
-    lse = torch.empty((p.heads, p.tokens), device=p.device, dtype=torch.float32)
-    a = build_args(p, out, lse)
-    a.num_splits = 1
     call(p, "fa_attn_fwd", a)
     return out, lse
+

@@ -16,8 +16,7 @@ num_splits is honoured.  fa_decode_fwd_noalloc plans the same way in C.
 """
 import torch
 
-from . import _lib
-from ._attention import _partials, build_args, f32_splits
+from ._attention import _partials, build_args, call, f32_splits, supported
 
 _MIN_WORKGROUPS = 1024
 _START_SPAN = 4096
@@ -73,16 +72,17 @@ def uses_gqa_kernel(p, rows=None):
     changes the split plan's workgroup estimate)."""
     page = p.k.shape[1] if p.paged else 0
     rows = p.max_q if rows is None else rows
-    small = p.dim_qk == 64 and gqa_pack(p, 1) == 2   # paired 64-dim heads take groups of 1-2 too
+    # Paired 64-dim heads take groups of 1-2 too, block-scaled caches any group.
+    small = p.block_scaled or (p.dim_qk == 64 and gqa_pack(p, 1) == 2)
     rows_ok = (p.heads // p.kv_heads >= _GQA_MIN_GROUP or small) if rows <= 1 else rows <= _GQA_MAX_ROWS
     out_dtype = p.out.dtype if p.out is not None else p.output_dtype
     if p.q.dtype == torch.float8_e4m3fn:
-        types_ok = rows <= 1 and out_dtype in (torch.float16, torch.bfloat16)
+        types_ok = rows <= 1 and out_dtype in (torch.float16, torch.bfloat16) and not p.block_scaled
     else:
         types_ok = p.q.dtype in (torch.float16, torch.bfloat16) and out_dtype == p.q.dtype
     return (rows_ok and types_ok and p.k.dtype == p.v.dtype and p.k.dtype in (p.q.dtype, torch.float8_e4m3fn)
             and p.dim_qk == p.dim_v and p.dim_qk in (64, 128) and p.alibi is None and p.mask is None
-            and page % 16 == 0)
+            and page % 16 == 0 and not (p.block_scaled and page // p.k_descale.shape[1] % 16))
 
 
 def gqa_pack(p, rows=1):
@@ -158,7 +158,7 @@ def decode(p, out, splits=None):
     if splits > 1:
         _partials(p, a, (splits, p.tokens, p.heads, p.dim_v), (splits, p.heads, p.tokens))
     a.num_splits = splits
-    _lib.call("fa_attn_fwd", a, p.device)
+    call(p, "fa_attn_fwd", a)
     return out, lse
 
 
@@ -179,7 +179,7 @@ def _run_split_kv(p, a, rows, splits=None):
     """fa_decode_fwd with the split plan (or `splits` splits) and partials
     (outputs [batch][S][rows][Hq][Dv], LSEs [batch][rows][Hq][S]); False when
     the decode kernels do not take the arguments."""
-    if not _lib.supported("fa_decode_supported", a):
+    if not supported(p, "fa_decode_supported", a):
         return False
     groups = decode_workgroups(p, rows)
     left = p.window[0]
@@ -188,5 +188,5 @@ def _run_split_kv(p, a, rows, splits=None):
     a.num_splits, a.split_span = splits, span
     if splits > 1:
         _partials(p, a, (p.batch, splits, rows, p.heads, p.dim_v), (p.batch, rows, p.heads, splits))
-    _lib.call("fa_decode_fwd", a, p.device)
+    call(p, "fa_decode_fwd", a)
     return True

@@ -187,8 +187,12 @@ def test_scale_bytes(device):
 
 @pytest.mark.parametrize("rows", [1, 4, 60])
 def test_nan_reaches_the_rows_that_see_it(device, rows):
-    """A NaN code, and a scale of 255, in one KV head: NaN for its query heads, the other heads as they were; hidden
-    ones (past the length, out of the window) reach nothing."""
+    """A NaN code, and a scale of 255, in one KV head: NaN for its query heads, the other heads at the bar; hidden ones
+    (past the length, out of the window) reach nothing.
+
+    Not bit for bit: heads that share matrix products with the NaN's, and rows whose tile holds the hidden one, run again
+    in fp32, without the rounding of probabilities to the queries' type, 2^-9 of each: at most 2^-9 sum p |v| of an
+    output, below the bar (2^-6.6) for these |v| < 4."""
     for dim in (64, 128):
         base = Call([rows, 1], [128 + rows, 90], 64, 16, 8, 4, dim)
         want, _ = base.gpu(device, causal=False)
@@ -202,7 +206,7 @@ def test_nan_reaches_the_rows_that_see_it(device, rows):
             out, _ = call.gpu(device, causal=False)
             assert out[:rows, 2:4].isnan().all()
             out[:rows, 2:4] = want[:rows, 2:4]
-            assert torch.equal(out, want)
+            assert ((out - want).abs() <= OUT_BAR[torch.bfloat16]).all()
         call = Call([rows, 1], [128 + rows, 90], 64, 16, 8, 4, dim)
         first, second = int(call.table[0, 0]), int(call.table[1, 1])
         for codes, scale in ((call.k, call.ks), (call.v, call.vs)):
@@ -212,7 +216,7 @@ def test_nan_reaches_the_rows_that_see_it(device, rows):
             scale.view(torch.uint8)[second, 2:] = 255
         out, _ = call.gpu(device, window_size=(100, 0))
         ref, _ = base.gpu(device, window_size=(100, 0))
-        assert torch.equal(out, ref)
+        assert ((out - ref).abs() <= OUT_BAR[torch.bfloat16]).all()
 
 
 def test_empty_requests_and_padding(device):
