@@ -43,7 +43,7 @@
 #ifndef FA_PREFILL_KERNEL_H
 #define FA_PREFILL_KERNEL_H
 
-#include "attn_common.h"
+#include "block_row.h"
 
 #include <climits>
 #include <type_traits>
@@ -123,13 +123,13 @@ FA_DEV u32x4 halves_swapped_if(u32x4 w, int swap) {
   return swap ? u32x4{w[2], w[3], w[0], w[1]} : w;
 }
 
-// 16 E4M3 codes -> 16 T values (dims 0..7 in lo, 8..15 in hi).
+// 16 E4M3 codes -> 16 T values times `scale` (dims 0..7 in lo, 8..15 in hi).
 template <typename T>
-FA_DEV void widen_fp8_16(u32x4 w, u32x4& lo, u32x4& hi) {
-  lo = u32x4{widen_fp8_pair<T, false>(w[0]), widen_fp8_pair<T, true>(w[0]), widen_fp8_pair<T, false>(w[1]),
-             widen_fp8_pair<T, true>(w[1])};
-  hi = u32x4{widen_fp8_pair<T, false>(w[2]), widen_fp8_pair<T, true>(w[2]), widen_fp8_pair<T, false>(w[3]),
-             widen_fp8_pair<T, true>(w[3])};
+FA_DEV void widen_fp8_16(u32x4 w, u32x4& lo, u32x4& hi, float scale = 1.0f) {
+  lo = u32x4{widen_fp8_pair<T, false>(w[0], scale), widen_fp8_pair<T, true>(w[0], scale),
+             widen_fp8_pair<T, false>(w[1], scale), widen_fp8_pair<T, true>(w[1], scale)};
+  hi = u32x4{widen_fp8_pair<T, false>(w[2], scale), widen_fp8_pair<T, true>(w[2], scale),
+             widen_fp8_pair<T, false>(w[3], scale), widen_fp8_pair<T, true>(w[3], scale)};
 }
 
 // Swap bits 2 and 3 of a row index (an involution).
@@ -253,12 +253,21 @@ FA_DEV int64_t request_by_rank(const fa_attn_args& a, int64_t rank, int lane) {
   return (int64_t)__builtin_ctzll(hit);
 }
 
+// The 16-key group of the rows that wave w widens in pass `it` of a 64 x DIM tile
+// by W waves: four 16-lane groups a wave, each 4 rows of one of DIM / 64 column
+// groups, so 4 q .. 4 q + 3 with q = (4 (W it + w) + i) / (DIM / 64), i = 0..3.
+template <int DIM, int W> FA_DEV int widen_group(int it, int w) {
+  static_assert(DIM == 64 || DIM == 128 || DIM == 256, "rows of a wave's pass in one 16-key group");
+  return (W * it + w) * 4 / (DIM / 64) / 4;
+}
+
 // V column parts of a tile: 256-dim heads run in 256/128 tiles, each work
 // item as two workgroups, one per 128-column half of V and of the output.
 template <int DQ, int DV> constexpr int prefill_vparts() { return DQ == 256 && DV == 128 ? 2 : 1; }
 
 struct PrefillShape {
   int n_qblocks;
+  int log2_block;  // block-scaled caches: block of slot s = s >> log2_block
   int log2_page;   // paged K/V: page of position p = p >> log2_page, slot p & (2^log2_page - 1)
   int compact;     // 1: workgroups map onto the compact work list
   int hp;          // query heads per workgroup (1 or 2, dividing the GQA group): W / hp waves per head
@@ -344,6 +353,31 @@ FA_DEV bool compact_item(const fa_attn_args& a, int slot, int xcd, int lane, int
   return false;
 }
 
+// The rows row0 + i of head h for each bit i of `bad`, over keys [begin, end), by
+// block_row, written as prefill_kernel writes them (both V parts write LSE and
+// their own columns).
+template <typename T, int D, bool TWO_PARTS>
+FA_DEV void rows_again(uint32_t bad, int64_t b, const RequestInfo& r, int kh, int h, int row0, int vpart, int split,
+                       int splits, int begin, int end, int lane) {
+  const fa_block_attn& a = block_arguments();
+  for (; bad; bad &= bad - 1) {
+    const int row = row0 + __builtin_ctz(bad);
+    const int64_t tq = (int64_t)r.q_begin + row;
+    const int64_t part = ((int64_t)split * a.total_q + tq) * a.heads_q + h;
+    const float lse = block_row<D / 64>(
+        a, b, r, kh, h, split, tq, row + r.k_len - r.q_len, begin, end, lane,
+        [&](int d) { return load_elem<T>(a.q, tq * a.q_stride[0] + (int64_t)h * a.q_stride[1] + d); },
+        [&](int d, float x) {
+          if (TWO_PARTS && d / (D / 2) != vpart) return;
+          if (splits > 1) a.partial_out[part * D + d] = x;
+          else store_elem<T>(a.out, tq * a.out_stride[0] + (int64_t)h * a.out_stride[1] + d, x);
+        });
+    if (lane != 0 || (TWO_PARTS && vpart)) continue;
+    if (splits > 1) a.partial_lse[((int64_t)split * a.heads_q + h) * a.total_q + tq] = lse;
+    else a.lse[(int64_t)h * a.lse_stride[0] + tq * a.lse_stride[1]] = lse != lse ? -INFINITY : lse;
+  }
+}
+
 // DQ / DV are the tile's head dims (multiples of 64); DQT / DVT <= them are
 // the tensors' own (multiples of 8): the query's extra dims load as zero,
 // their K columns are never multiplied (K-steps past DQT are skipped, a half
@@ -361,13 +395,21 @@ FA_DEV bool compact_item(const fa_attn_args& a, int slot, int xcd, int lane, int
 // MK: vLLM mask kind (a.mask_kind; 0 none): each row's visible keys are at
 // most two key ranges (see mask_ranges below); causality and the window
 // fields do not apply, as in the reference (kernels/attention.metal:29-45).
+// BLOCK: a block-scaled cache (E4M3 codes, blocks of a power of two >= 16 keys):
+// the widening passes, where a wave's rows of a pass lie in one 16-key group,
+// take that group's power of two into the conversion at no cost; its bytes are
+// loaded a tile ahead, with the codes.  Rows whose sums are not finite (a NaN in
+// a value that another row of the tile sees; fp16 past its range) run again by
+// block_row.
 // SPLIT: a.num_splits workgroups (blockIdx.y; request_splits of them at work)
 // share each work item's key tiles evenly and write fp32 partials for
 // prefill_merge_kernel: for grids that leave CUs idle (a chunk of a few hundred
 // rows behind a long prefix).
 template <typename T, int DQ, int DV, int W, int NB, int MINB, bool CAUSAL, bool CAP, bool WIN, int DQT = DQ,
-          int DVT = DV, typename KT = T, bool ALIBI = false, typename QT = T, int MK = 0, bool SPLIT = false>
-__global__ __launch_bounds__(64 * W, MINB) void prefill_kernel(const fa_attn_args a, const PrefillShape shp) {
+          int DVT = DV, typename KT = T, bool ALIBI = false, typename QT = T, int MK = 0, bool SPLIT = false,
+          bool BLOCK = false>
+__global__ __launch_bounds__(64 * W, MINB) void prefill_kernel(const typename AttnArgsOf<BLOCK>::type a,
+                                                               const PrefillShape shp) {
   static_assert(MK == 0 || (!CAUSAL && !WIN && !ALIBI), "mask kinds carry their own causality and windows");
   constexpr bool GEN = WIN || MK != 0;   // per-stage hot / masked decisions (no closed-form hot loop)
   constexpr bool FP8 = KT::id == FA_E4M3;
@@ -380,6 +422,7 @@ __global__ __launch_bounds__(64 * W, MINB) void prefill_kernel(const fa_attn_arg
                                                       (DQ == 256 && DV == 128))),
                 "FP8 K/V tiles: 64/128/256-dim heads (256-dim: also as 256/128 V halves)");
   static_assert(!FQ || FP8, "E4M3 queries: E4M3 K/V");
+  static_assert(!BLOCK || (FP8 && !FQ && !ALIBI), "block scales: E4M3 K/V, 16-bit queries, no ALiBi");
   constexpr int BM = 32 * NB * W;              // query rows per workgroup
   constexpr int KST = DQ / 16;                 // k-steps of the QK^T MFMA
   constexpr int KSTT = (DQT + 15) / 16;        // k-steps holding real dims
@@ -756,7 +799,31 @@ __global__ __launch_bounds__(64 * W, MINB) void prefill_kernel(const fa_attn_arg
   const int k8row = ((KR8 * wave_u) & 15) + lane / (DQ / 16), v8row = ((VR8 * wave_u) & 15) + lane / (DV / 16);
   const int k8off = k8row * (int)krow_b + ((lane % (DQ / 16)) ^ stage_rows<DQ>(k8row)) * 16;
   const int v8off = v8row * (int)vrow_b + ((lane % (DV / 16)) ^ stage_rows<DV>(v8row)) * 16;
+  // BLOCK: the scale bytes of the staged tile's rows that this wave widens, one
+  // per pass (widen_k_rows, widen_v_rows): pass `it` covers the 64 W / DIM rows
+  // from 64 W / DIM * 16 / W ... of one 16-key group.
+  constexpr int KIT = BLOCK ? DQ / (16 * W) : 1, VIT = BLOCK ? DV / (16 * W) : 1;
+  uint32_t kbyte[KIT], vbyte[VIT];
+  auto load_scales = [&](int tile) {
+    if constexpr (BLOCK) {
+      auto byte_of = [&](int which, int group) {
+        const int key0 = tile * PF_BN + 16 * group;
+        uint32_t e = 127;
+        if (key0 < r.k_len) {
+          const int64_t blk = load_invariant_i32(trow, (int64_t)(key0 >> lp) * bt1);
+          const int64_t* st = a.scale_stride[which];
+          e = a.scale[which][blk * st[0] + (int64_t)((key0 & pmask) >> shp.log2_block) * st[1] + kh * st[2]];
+        }
+        return e;
+      };
+#pragma unroll
+      for (int it = 0; it < KIT; ++it) kbyte[it] = byte_of(0, widen_group<DQ, W>(it, wave_u));
+#pragma unroll
+      for (int it = 0; it < VIT; ++it) vbyte[it] = byte_of(1, widen_group<DV, W>(it, wave_u));
+    }
+  };
   auto dma_fp8 = [&](int tile) {
+    load_scales(tile);
 #pragma unroll
     for (int i = 0; i < 64 / KR8 / W; ++i) {
       const int n = wave_u + W * i;
@@ -802,7 +869,7 @@ __global__ __launch_bounds__(64 * W, MINB) void prefill_kernel(const fa_attn_arg
       const int r = 4 * q + (l16 >> 2), u = 4 * g + m, rho = sigma(r), sw = (rho >> 1) & 7, up = r & 1;
       u32x4 first, second;
       widen_fp8_16<T>(halves_swapped_if(*(const u32x4*)(stk + r * DQ + 16 * (u ^ stage_rows<DQ>(r))), up), first,
-                      second);
+                      second, BLOCK ? e8m0_to_f32(kbyte[BLOCK ? it : 0]) : 1.0f);
       char* const row = kbuf0 + buf * KTILE + g * PF_GROUP_BYTES + rho * 128;
       *(u32x4*)(row + ((2 * m + up) ^ sw) * 16) = first;
       *(u32x4*)(row + ((2 * m + 1 - up) ^ sw) * 16) = second;
@@ -817,7 +884,7 @@ __global__ __launch_bounds__(64 * W, MINB) void prefill_kernel(const fa_attn_arg
       const int r = 4 * ((it * GPI + (t >> 4)) / NC) + (l16 >> 2);
       u32x4 first, second;
       widen_fp8_16<T>(halves_swapped_if(*(const u32x4*)(stage + r * DV + 16 * (u ^ stage_rows<DV>(r))), up), first,
-                      second);
+                      second, BLOCK ? e8m0_to_f32(vbyte[BLOCK ? it : 0]) : 1.0f);
       char* const dst = vbuf0 + buf * VTILE + blk * PF_VBLOCK_BYTES + r * 64 + 32 * h;
       *(u32x4*)(dst + 16 * up) = first;
       *(u32x4*)(dst + 16 * (1 - up)) = second;
@@ -1357,7 +1424,21 @@ __global__ __launch_bounds__(64 * W, MINB) void prefill_kernel(const fa_attn_arg
   for (int nb = 0; nb < NB; ++nb) {
     const float lt = sum_hh(l_run[nb]);
     const int row = wq0 + 32 * nb + l32;
-    if (row < r.q_len) {
+    bool again = false;
+    if constexpr (BLOCK) {
+      float probe = lt * 0.0f;
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) probe = fmaf(o[nb][db][i], 0.0f, probe);
+      const uint64_t bad = __ballot(probe != 0.0f && row < r.q_len);   // (NaN; lanes l32 and l32 + 32 hold a row)
+      if (__builtin_expect(bad != 0, 0)) {
+        again = ((uint32_t)bad | (uint32_t)(bad >> 32)) >> l32 & 1;
+        rows_again<T, DQ, TWO_PARTS>((uint32_t)bad | (uint32_t)(bad >> 32), b, r, kh, h, wq0 + 32 * nb, vpart, split, splits,
+                                     SPLIT ? tile0 * PF_BN : 0, kv_end, lane);
+      }
+    }
+    if (row < r.q_len && !again) {
       const float inv = lt > 0.0f ? vdsc / lt : 0.0f;
       const int64_t tq = (int64_t)r.q_begin + row;
       if (SPLIT && splits > 1) {
@@ -1423,14 +1504,15 @@ constexpr size_t lds_bytes() {
   return 2 * (size_t)(DQ / 64 + DV / 64) * PF_GROUP_BYTES;
 }
 
-using PrefillKernel = void (*)(fa_attn_args, PrefillShape);
-
-struct PrefillChoice {
-  PrefillKernel kern;
+template <typename A>
+struct PrefillChoiceOf {
+  void (*kern)(A, PrefillShape);
   int bm, threads;
   size_t lds;
   int vparts;   // workgroups per work item, one per DV-column part of the head (prefill_vparts)
 };
+using PrefillKernel = void (*)(fa_attn_args, PrefillShape);
+using PrefillChoice = PrefillChoiceOf<fa_attn_args>;
 
 // score: 0 plain, 1 softcap, 2 ALiBi, 3 softcap then ALiBi; mk: vLLM
 // mask kind (0 none; instantiated for unpadded head dims without ALiBi, not
@@ -1623,6 +1705,52 @@ PrefillChoice pick_split(int64_t dq, int64_t dv, bool causal, bool cap) {
   }
   return PrefillChoice{nullptr, 0, 0, 0, 0};
 }
+
+// Block-scaled caches: the E4M3 tiles at 64, 128 and 256 dims (256 as V halves)
+// with softcap, windows, the vLLM mask kinds (without softcap) and key splits
+// (without windows and mask kinds).
+template <typename T, int DQ, int DV, bool CAUSAL>
+PrefillChoiceOf<fa_block_attn> pick_tile_block(bool cap, bool win, int mk, bool split) {
+  using S = PrefillTile<DQ, DV>;
+  PrefillChoiceOf<fa_block_attn> c{nullptr, 0, 0, 0, 0};
+  if (mk != 0) {
+    if constexpr (!CAUSAL) {
+      if (!cap && !split)
+        c.kern = mk == 1 ? prefill_kernel<T, DQ, DV, S::W, S::NB, S::MINB_WIN, false, false, false, DQ, DV, E4M3T, false, T, 1, false, true>
+                         : prefill_kernel<T, DQ, DV, S::W, S::NB, S::MINB_WIN, false, false, false, DQ, DV, E4M3T, false, T, 2, false, true>;
+    }
+  } else if (split) {
+    if (win) return c;
+    c.kern = cap ? prefill_kernel<T, DQ, DV, S::W, S::NB, S::MINB, CAUSAL, true, false, DQ, DV, E4M3T, false, T, 0, true, true>
+                 : prefill_kernel<T, DQ, DV, S::W, S::NB, S::MINB, CAUSAL, false, false, DQ, DV, E4M3T, false, T, 0, true, true>;
+  } else if (win) {
+    c.kern = cap ? prefill_kernel<T, DQ, DV, S::W, S::NB, S::MINB_WIN, CAUSAL, true, true, DQ, DV, E4M3T, false, T, 0, false, true>
+                 : prefill_kernel<T, DQ, DV, S::W, S::NB, S::MINB_WIN, CAUSAL, false, true, DQ, DV, E4M3T, false, T, 0, false, true>;
+  } else {
+    c.kern = cap ? prefill_kernel<T, DQ, DV, S::W, S::NB, S::MINB, CAUSAL, true, false, DQ, DV, E4M3T, false, T, 0, false, true>
+                 : prefill_kernel<T, DQ, DV, S::W, S::NB, S::MINB, CAUSAL, false, false, DQ, DV, E4M3T, false, T, 0, false, true>;
+  }
+  c.bm = 32 * S::NB * S::W;
+  c.threads = 64 * S::W;
+  c.lds = lds_bytes<DQ, DV>() + 64 * (size_t)(DQ + DV);   // + the staging tile
+  c.vparts = prefill_vparts<DQ, DV>();
+  return c;
+}
+
+template <typename T>
+PrefillChoiceOf<fa_block_attn> pick_block(int64_t d, bool causal, bool cap, bool win, int mk, bool split) {
+  const bool c = causal && mk == 0;   // mask kinds carry their own causality
+  switch (d) {
+    case 64: return c ? pick_tile_block<T, 64, 64, true>(cap, win, mk, split) : pick_tile_block<T, 64, 64, false>(cap, win, mk, split);
+    case 128: return c ? pick_tile_block<T, 128, 128, true>(cap, win, mk, split) : pick_tile_block<T, 128, 128, false>(cap, win, mk, split);
+    case 256: return c ? pick_tile_block<T, 256, 128, true>(cap, win, mk, split) : pick_tile_block<T, 256, 128, false>(cap, win, mk, split);
+    default: return {nullptr, 0, 0, 0, 0};
+  }
+}
+
+// Defined in prefill_inst_block_{bf16,f16}.hip.
+PrefillChoiceOf<fa_block_attn> pick_block_bf16(int64_t d, bool causal, bool cap, bool win, int mk, bool split);
+PrefillChoiceOf<fa_block_attn> pick_block_f16(int64_t d, bool causal, bool cap, bool win, int mk, bool split);
 
 // Defined in prefill_inst_split_{16,fp8,fp8q}.hip; bf16: the kernel's 16-bit
 // type (the query's, or the output's with E4M3 queries).

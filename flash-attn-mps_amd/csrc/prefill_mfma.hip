@@ -166,25 +166,22 @@ bool prefill_ok(const fa_attn_args& a) {
   return true;
 }
 
-}  // namespace
-
-extern "C" int fa_prefill_supported(const fa_attn_args* a) {
-  return a != nullptr && prefill_ok(fa_bounded(*a));
+// What the kernel takes of a block-scaled cache beside that: blocks of a power
+// of two that hold whole 16-key groups, 16-bit queries, no ALiBi, mask kinds
+// without softcap.
+bool block_ok(const fa_block_attn& a) {
+  return prefill_ok(a) && a.page_size && a.q_dtype != FA_E4M3 && !a.alibi && a.block % 16 == 0 &&
+         (a.block & (a.block - 1)) == 0 && !(a.mask_kind != 0 && a.softcap > 0.0f);
 }
 
-extern "C" int fa_prefill_fwd(const fa_attn_args* args, void* stream) {
-  int rc = fa_validate_attn(args, "fa_prefill_fwd");
-  if (rc) return rc;
-  const fa_attn_args bounded = fa_bounded(*args), *a = &bounded;
-  if (!prefill_ok(*a)) {
-    fa_set_error("fa_prefill_fwd: combination not supported by the MFMA kernel");
-    return FA_ERR_UNSUPPORTED;
-  }
+// Launch the kernel of `ch`, and the merge with key splits, for checked arguments.
+template <typename A>
+int launch_prefill(const A* a, const PrefillChoiceOf<A>& ch, int log2_block, void* stream, const char* who) {
   if (a->total_q == 0) return FA_OK;
-  FA_REQUIRE(a->max_seqlen_q >= 1, "fa_prefill_fwd: max_seqlen_q must be positive");
-  PrefillChoice ch = select_prefill(*a);
-  FA_REQUIRE(ch.kern != nullptr && ch.vparts >= 1, "fa_prefill_fwd: no kernel instance for these arguments");
+  FA_REQUIRE(a->max_seqlen_q >= 1, "%s: max_seqlen_q must be positive", who);
+  FA_REQUIRE(ch.kern != nullptr && ch.vparts >= 1, "%s: no kernel instance for these arguments", who);
   PrefillShape shp;
+  shp.log2_block = log2_block;
   // Query heads per workgroup: two heads of a KV head share each workgroup's
   // K/V tiles when the GQA group is even.
   shp.hp = (a->heads_q / a->heads_k) % 2 == 0 ? 2 : 1;
@@ -215,28 +212,64 @@ extern "C" int fa_prefill_fwd(const fa_attn_args* args, void* stream) {
   // V column parts: each work item runs as vparts workgroups (blocks is a
   // multiple of 8, as the kernel's 16-block interleave of the parts needs).
   blocks *= ch.vparts;
-  FA_REQUIRE(blocks <= 0x7fffffffll, "fa_prefill_fwd: grid too large");
+  FA_REQUIRE(blocks <= 0x7fffffffll, "%s: grid too large", who);
   const bool split = a->num_splits > 1;
   FA_REQUIRE(!split || (a->partial_out && a->partial_lse && aligned16(a->partial_out)),
-             "fa_prefill_fwd: splits need partial buffers, the outputs' 16-byte aligned");
+             "%s: splits need partial buffers, the outputs' 16-byte aligned", who);
   // The merge's rows per request: max_seqlen_q may be far above any request's.
   const int64_t merge_rows = (a->max_seqlen_q < a->total_q ? a->max_seqlen_q : a->total_q) * a->heads_q;
-  FA_REQUIRE(!split || (a->batch <= 65535 && merge_rows <= 0x7fffffffll), "fa_prefill_fwd: split grid too large");
+  FA_REQUIRE(!split || (a->batch <= 65535 && merge_rows <= 0x7fffffffll), "%s: split grid too large", who);
   hipError_t err = hipFuncSetAttribute((const void*)ch.kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)ch.lds);
   if (err != hipSuccess) {
-    fa_set_error("fa_prefill_fwd: cannot reserve %zu bytes of LDS: %s", ch.lds, hipGetErrorString(err));
+    fa_set_error("%s: cannot reserve %zu bytes of LDS: %s", who, ch.lds, hipGetErrorString(err));
     return FA_ERR_LAUNCH;
   }
   // Splits are the slow grid dimension and `blocks` a multiple of 8, so a
   // work item's splits stay on its XCD.
   hipLaunchKernelGGL(ch.kern, dim3((unsigned)blocks, (unsigned)(split ? a->num_splits : 1)), dim3(ch.threads), ch.lds,
                      (hipStream_t)stream, *a, shp);
-  rc = fa_check_launch("fa_prefill_fwd");
+  const int rc = fa_check_launch(who);
   if (rc || !split) return rc;
   void (*merge)(const fa_attn_args) = a->head_dim_v == 64    ? prefill_merge_kernel<1, 8>
                                       : a->head_dim_v == 128 ? prefill_merge_kernel<2, 8>
                                                              : prefill_merge_kernel<4, 4>;
   hipLaunchKernelGGL(merge, dim3((unsigned)fa_ceil_div(merge_rows, 4), (unsigned)a->batch), dim3(256), 0,
                      (hipStream_t)stream, *a);
-  return fa_check_launch("fa_prefill_fwd");
+  return fa_check_launch(who);
+}
+
+}  // namespace
+
+extern "C" int fa_prefill_supported(const fa_attn_args* a) {
+  return a != nullptr && prefill_ok(fa_bounded(*a));
+}
+
+extern "C" int fa_prefill_fwd(const fa_attn_args* args, void* stream) {
+  const int rc = fa_validate_attn(args, "fa_prefill_fwd");
+  if (rc) return rc;
+  const fa_attn_args a = fa_bounded(*args);
+  if (!prefill_ok(a)) {
+    fa_set_error("fa_prefill_fwd: combination not supported by the MFMA kernel");
+    return FA_ERR_UNSUPPORTED;
+  }
+  return launch_prefill(&a, select_prefill(a), 0, stream, "fa_prefill_fwd");
+}
+
+extern "C" int fa_block_prefill_supported(const fa_block_attn_args* args) {
+  fa_block_attn a;
+  return fa_block_arguments(args, &a) && block_ok(a);
+}
+
+extern "C" int fa_block_prefill_fwd(const fa_block_attn_args* args, void* stream) {
+  const char* who = "fa_block_prefill_fwd";
+  fa_block_attn a;
+  const int rc = fa_validate_block(args, &a, who);
+  if (rc) return rc;
+  if (!block_ok(a)) {
+    fa_set_error("%s: combination not supported by the MFMA kernel", who);
+    return FA_ERR_UNSUPPORTED;
+  }
+  const PrefillChoiceOf<fa_block_attn> ch = (a.q_dtype == FA_BF16 ? pick_block_bf16 : pick_block_f16)(
+      a.head_dim_qk, a.causal != 0, a.softcap > 0.0f, a.mask_kind == 0 && window_set(a), a.mask_kind, a.num_splits > 1);
+  return launch_prefill(&a, ch, __builtin_ctz((unsigned)a.block), stream, who);
 }

@@ -142,7 +142,7 @@ def _fits_prefill(p, out):
     or E4M3 K/V with output in the query's type, or E4M3 queries over E4M3 K/V
     with fp16/bf16 output (S on the FP8 MFMA).  Deterministic calls qualify:
     prefill_splits keeps them, and num_splits=1, at one split."""
-    if p.splits not in (0, 1) or p.block_scaled:
+    if p.splits not in (0, 1):
         return False
     fp8 = torch.float8_e4m3fn
     if p.k.dtype != p.v.dtype:

@@ -202,6 +202,8 @@ ENTRY_POINTS = {
     "fa_paged_append": (PagedAppendArgs, ctypes.c_int),
     "fa_block_decode_supported": (BlockAttnArgs, ctypes.c_int),
     "fa_block_decode_fwd": (BlockAttnArgs, ctypes.c_int),
+    "fa_block_prefill_supported": (BlockAttnArgs, ctypes.c_int),
+    "fa_block_prefill_fwd": (BlockAttnArgs, ctypes.c_int),
     "fa_block_attn_fwd": (BlockAttnArgs, ctypes.c_int),
     "fa_decode_supported": (AttnArgs, ctypes.c_int),
     "fa_decode_fwd": (AttnArgs, ctypes.c_int),

@@ -362,11 +362,15 @@ int fa_prefill_fwd(const fa_attn_args* args, void* stream);
  * partial_lse [S, Hq, T] and merges into out/lse. */
 int fa_attn_fwd(const fa_attn_args* args, void* stream);
 
-/* fa_decode_* and fa_attn_fwd over a block-scaled cache, with the same plans,
- * partials and errors.  Decode: the matrix-core kernel, any group, head dims 64
- * and 128, 16-bit queries, blocks that are multiples of 16. */
+/* fa_decode_*, fa_prefill_* and fa_attn_fwd over a block-scaled cache, with the
+ * same plans, partials and errors.  Decode: the matrix-core kernel, any group,
+ * head dims 64 and 128.  Prefill: head dims 64, 128 and 256, no ALiBi, mask kinds
+ * without softcap.  Both: 16-bit queries, blocks that are multiples of 16
+ * (prefill: powers of two). */
 int fa_block_decode_supported(const fa_block_attn_args* args);
 int fa_block_decode_fwd(const fa_block_attn_args* args, void* stream);
+int fa_block_prefill_supported(const fa_block_attn_args* args);
+int fa_block_prefill_fwd(const fa_block_attn_args* args, void* stream);
 int fa_block_attn_fwd(const fa_block_attn_args* args, void* stream);
 
 int fa_merge_pair(const fa_merge_pair_args* args, void* stream);
