@@ -10,14 +10,17 @@
 // small ones.
 //
 // A unit is W pairs of a row (W = 16 bytes of elements, or one pair where
-// strides, dims or alignment forbid vectors): two pieces of W elements, next to
+// strides, dims or alignment, of the tables too, forbid vectors): two pieces of W elements, next to
 // each other for interleaved pairs, half_rot apart otherwise; dims that do not
 // rotate are copied two pieces a unit.  A lane keeps its unit over all the
-// heads it takes, so cos and sin are loaded once per token and lane.
+// heads it takes, so cos and sin are loaded once per token and lane.  A wave
+// works on one token, or on one block of one head: what follows from those
+// (request, position, page) is scalar.
 //
 // Block-scaled caches: one wave owns a (block of tokens, head) of K or V, so
 // the block's largest magnitude, its scale and its rows need no other wave, and
-// the result does not depend on any order.
+// the result does not depend on any order.  The rows stay in registers between
+// the two passes that this takes, up to HOLD rows a lane.
 #include "attn_common.h"
 
 namespace {
@@ -44,10 +47,12 @@ struct AppendParams {
   int64_t block_stride[2][3];
   const int32_t *cu, *used, *table;
   int64_t cu_stride, used_stride, bt_stride[2];
-  int64_t tokens, page_size, num_pages, table_cols;
-  int32_t batch, block, lanes;   // lanes: units of a row handled at once
-  int32_t row_heads;             // heads of a token that run as rows (parts in order)
-  uint32_t block_waves;          // workgroups 0 .. ceil(block_waves / 4) - 1 own blocks
+  int64_t tokens, num_pages, table_cols;
+  int32_t batch, page_size, block;   // page_size: clipped to 32 bits, as positions are
+  int32_t lanes;                     // units of a row handled at once
+  int32_t passes[3];                 // passes of 64 / lanes heads over each part's rows (0: not as rows)
+  uint32_t token_waves;              // waves of a token
+  uint32_t block_waves;              // workgroups 0 .. ceil(block_waves / 4) - 1 own blocks
 };
 
 // The largest i < n with key(i) <= target (key nondecreasing), -1 if none: 64
@@ -63,94 +68,185 @@ FA_DEV int last_at_most(int n, int64_t target, int lane, F key) {
     lo += count * step;
     end = min(end, lo + step - 1);
   }
-  return lo;
+  return __builtin_amdgcn_readfirstlane(lo);
 }
 
-FA_DEV int64_t cu_at(const AppendParams& p, int b) { return p.cu[b * p.cu_stride]; }
+FA_DEV int cu_at(const AppendParams& p, int b) { return p.cu[b * p.cu_stride]; }
+FA_DEV int cu_of(const AppendParams& p, int b) { return load_invariant_i32(p.cu, b * p.cu_stride); }   // uniform b
 
-// One page of the cache that position `pos` of request b lies in; -1: none.
-FA_DEV int64_t page_of(const AppendParams& p, int b, int64_t pos) {
-  if (pos < 0) return -1;
-  const int64_t column = pos / p.page_size;
-  if (column >= p.table_cols) return -1;
-  const int64_t page = p.table[b * p.bt_stride[0] + column * p.bt_stride[1]];
-  return page >= 0 && page < p.num_pages ? page : -1;
+// Where position `pos` of request b lies; page -1: nowhere.
+struct Place {
+  int64_t page;
+  int row;
+};
+
+FA_DEV Place place_of(const AppendParams& p, int b, int64_t pos) {
+  Place x{-1, 0};
+  if (pos < 0 || pos > INT32_MAX) return x;
+  const uint32_t column = (uint32_t)pos / (uint32_t)p.page_size;
+  if ((int64_t)column >= p.table_cols) return x;
+  const int64_t page = load_invariant_i32(p.table, b * p.bt_stride[0] + (int64_t)column * p.bt_stride[1]);
+  if (page < 0 || page >= p.num_pages) return x;
+  x.page = page;
+  x.row = (int)((uint32_t)pos - column * (uint32_t)p.page_size);
+  return x;
 }
 
-// The row of the cos/sin tables for pair i of token t; -1: none.
-FA_DEV int64_t trig_row(const AppendParams& p, int64_t t, int64_t cache_pos, int i) {
-  int64_t pos = cache_pos;
-  if (p.rot.positions) {
-    const int axis = (int)(p.rot.pair_axis[i >> 5] >> (2 * (i & 31))) & 3;
-    const int64_t at = axis * p.rot.position_stride[0] + t * p.rot.position_stride[1];
-    pos = p.rot.position_dtype == FA_I64 ? ((const int64_t*)p.rot.positions)[at] : ((const int32_t*)p.rot.positions)[at];
+FA_DEV uint32_t pair_axes(const AppendParams& p, int i) {
+  uint64_t w = p.rot.pair_axis[0];
+#pragma unroll
+  for (int k = 1; k < 8; ++k) w = i >> 5 == k ? p.rot.pair_axis[k] : w;
+  return (uint32_t)(w >> (2 * (i & 31)));
+}
+
+FA_DEV int64_t position_of(const AppendParams& p, int64_t t, int axis) {
+  const int64_t at = axis * p.rot.position_stride[0] + t * p.rot.position_stride[1];
+  return p.rot.position_dtype == FA_I64 ? ((const int64_t*)p.rot.positions)[at] : ((const int32_t*)p.rot.positions)[at];
+}
+
+// cos and sin of pairs i .. i + W - 1 at row `row` of the tables (W > 1: aligned
+// pieces of contiguous rows); NaN without one.
+template <int W>
+FA_DEV void load_row(const AppendParams& p, int64_t row, int i, float (&c)[W], float (&s)[W]) {
+#pragma unroll
+  for (int j = 0; j < W; ++j) c[j] = s[j] = __builtin_nanf("");
+  if (row < 0 || row >= p.rot.table_rows) return;
+  const int64_t ca = row * p.rot.cos_stride[0], sa = row * p.rot.sin_stride[0];
+  if constexpr (W == 1) {
+    c[0] = load_any(p.rot.cos_table, ca + i * p.rot.cos_stride[1], p.rot.trig_dtype);
+    s[0] = load_any(p.rot.sin_table, sa + i * p.rot.sin_stride[1], p.rot.trig_dtype);
+  } else if (p.rot.trig_dtype == FA_F32) {
+#pragma unroll
+    for (int j = 0; j < W; j += 4) {
+      const float4 x = *(const float4*)((const float*)p.rot.cos_table + ca + i + j);
+      const float4 y = *(const float4*)((const float*)p.rot.sin_table + sa + i + j);
+      c[j] = x.x, c[j + 1] = x.y, c[j + 2] = x.z, c[j + 3] = x.w;
+      s[j] = y.x, s[j + 1] = y.y, s[j + 2] = y.z, s[j + 3] = y.w;
+    }
+  } else {
+    const bool bf = p.rot.trig_dtype == FA_BF16;
+#pragma unroll
+    for (int j = 0; j < W; j += 4) {
+      const uint2 x = *(const uint2*)((const uint16_t*)p.rot.cos_table + ca + i + j);
+      const uint2 y = *(const uint2*)((const uint16_t*)p.rot.sin_table + sa + i + j);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t u = (k & 2 ? x.y : x.x) >> (16 * (k & 1)) & 0xffffu, v = (k & 2 ? y.y : y.x) >> (16 * (k & 1)) & 0xffffu;
+        c[j + k] = bf ? bf16_bits_to_f32(u) : f16_bits_to_f32(u);
+        s[j + k] = bf ? bf16_bits_to_f32(v) : f16_bits_to_f32(v);
+      }
+    }
   }
-  return pos >= 0 && pos < p.rot.table_rows ? pos : -1;
 }
 
-// cos and sin of pairs i .. i + W - 1 of token t.
+// cos and sin of pairs i .. i + W - 1 (i a multiple of W) of token t: a row for
+// each axis that they have, which is one unless axes alternate.
 template <int W>
 FA_DEV void load_trig(const AppendParams& p, int64_t t, int64_t cache_pos, int i, float (&c)[W], float (&s)[W]) {
+  const uint32_t axes = p.rot.positions ? pair_axes(p, i) : 0;
+  uint32_t todo = 0;
 #pragma unroll
-  for (int j = 0; j < W; ++j) {
-    const int64_t row = trig_row(p, t, cache_pos, i + j);
-    c[j] = s[j] = __builtin_nanf("");
-    if (row >= 0) {
-      c[j] = load_any(p.rot.cos_table, row * p.rot.cos_stride[0] + (i + j) * p.rot.cos_stride[1], p.rot.trig_dtype);
-      s[j] = load_any(p.rot.sin_table, row * p.rot.sin_stride[0] + (i + j) * p.rot.sin_stride[1], p.rot.trig_dtype);
+  for (int j = 0; j < W; ++j) todo |= 1u << (axes >> (2 * j) & 3);
+  while (todo) {
+    const uint32_t axis = (uint32_t)__builtin_ctz(todo);
+    todo &= todo - 1;
+    float ca[W], sa[W];
+    load_row<W>(p, p.rot.positions ? position_of(p, t, axis) : cache_pos, i, ca, sa);
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      const bool own = (axes >> (2 * j) & 3) == axis;
+      c[j] = own ? ca[j] : c[j];
+      s[j] = own ? sa[j] : s[j];
     }
   }
 }
 
 // The elements at which unit u's two pieces start; the second is -1 where the
 // row ends before it.
+struct Unit {
+  int lo, hi;
+  bool turns;
+};
+
 template <int W>
-FA_DEV void unit_places(const AppendRows& r, bool interleaved, int u, int& lo, int& hi, bool& turns) {
+FA_DEV Unit unit_of(const AppendRows& r, bool interleaved, int u) {
   const int rotated = r.half / W;
-  turns = u < rotated;
-  if (turns) {
-    lo = interleaved ? 2 * u * W : u * W;
-    hi = interleaved ? lo + W : r.half + lo;
+  Unit x;
+  x.turns = u < rotated;
+  if (x.turns) {
+    x.lo = interleaved ? 2 * u * W : u * W;
+    x.hi = interleaved ? x.lo + W : r.half + x.lo;
   } else {
-    lo = 2 * r.half + (u - rotated) * 2 * W;
-    hi = lo + W < r.dim ? lo + W : -1;
+    x.lo = 2 * r.half + (u - rotated) * 2 * W;
+    x.hi = x.lo + W < r.dim ? x.lo + W : -1;
   }
+  return x;
 }
 
-template <typename XT, int W> struct Piece { typename XT::storage e[W]; };
+// W elements as they are stored: 16 bytes, or one element's bits.
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+template <int W> struct PieceOf { using type = u32x4; };
+template <> struct PieceOf<1> { using type = uint32_t; };
+template <int W> using Piece = typename PieceOf<W>::type;
 
 template <typename XT, int W>
-FA_DEV Piece<XT, W> load_piece(const void* x, int64_t at, int64_t stride) {
+FA_DEV Piece<W> load_piece(const void* x, int64_t at) {
   using S = typename XT::storage;
-  Piece<XT, W> r;
   if constexpr (W > 1) {
     static_assert(W * sizeof(S) == 16, "vector pieces");
-    r = __builtin_bit_cast(Piece<XT, W>, *(const uint4*)((const S*)x + at));
+    return *(const u32x4*)((const S*)x + at);
+  } else if constexpr (sizeof(S) == 4) {
+    return ((const uint32_t*)x)[at];
   } else {
-    r.e[0] = ((const S*)x)[at];
+    return ((const S*)x)[at];
   }
-  return r;
 }
 
 template <typename XT, int W>
-FA_DEV void store_piece(void* x, int64_t at, const Piece<XT, W>& v) {
+FA_DEV void store_piece(void* x, int64_t at, Piece<W> v) {
   using S = typename XT::storage;
-  if constexpr (W > 1) *(uint4*)((S*)x + at) = __builtin_bit_cast(uint4, v);
-  else ((S*)x)[at] = v.e[0];
+  if constexpr (W > 1) *(u32x4*)((S*)x + at) = v;
+  else if constexpr (sizeof(S) == 4) ((uint32_t*)x)[at] = v;
+  else ((S*)x)[at] = (S)v;
+}
+
+template <typename XT>
+FA_DEV float value_of_bits(uint32_t bits) {
+  if constexpr (XT::id == FA_F32) return __uint_as_float(bits);
+  else if constexpr (XT::id == FA_BF16) return bf16_bits_to_f32(bits);
+  else return f16_bits_to_f32(bits);
+}
+
+template <typename XT>
+FA_DEV uint32_t bits_of_value(float f) {
+  if constexpr (XT::id == FA_F32) return __float_as_uint(f);
+  else if constexpr (XT::id == FA_BF16) return f32_to_bf16_bits(f);
+  else return f32_to_f16_bits(f);
 }
 
 template <typename XT, int W>
-FA_DEV void widen(const Piece<XT, W>& v, float (&f)[W]) {
+FA_DEV void widen(Piece<W> v, float (&f)[W]) {
+  if constexpr (W == 1) {
+    f[0] = value_of_bits<XT>(v);
+  } else {
 #pragma unroll
-  for (int j = 0; j < W; ++j) f[j] = load_elem<XT>(v.e, j);
+    for (int j = 0; j < W; ++j)
+      f[j] = value_of_bits<XT>(XT::bytes == 4 ? v[j % 4] : v[j / 2] >> (16 * (j & 1)) & 0xffffu);
+  }
 }
 
 template <typename XT, int W>
-FA_DEV Piece<XT, W> narrow(const float (&f)[W]) {
-  Piece<XT, W> v;
+FA_DEV Piece<W> narrow(const float (&f)[W]) {
+  if constexpr (W == 1) {
+    return bits_of_value<XT>(f[0]);
+  } else {
+    u32x4 v;
 #pragma unroll
-  for (int j = 0; j < W; ++j) store_elem<XT>(v.e, j, f[j]);
-  return v;
+    for (int j = 0; j < 4; ++j)
+      v[j] = XT::bytes == 4 ? bits_of_value<XT>(f[j % W])
+                            : bits_of_value<XT>(f[2 * j % W]) | bits_of_value<XT>(f[(2 * j + 1) % W]) << 16;
+    return v;
+  }
 }
 
 // The W pairs of a unit turned; lo and hi are its pieces.
@@ -176,90 +272,134 @@ FA_DEV void turn(float (&lo)[W], float (&hi)[W], const float (&c)[W], const floa
   }
 }
 
-// W values as E4M3 codes at element `at` (16-byte pieces: W contiguous codes).
+// W values as contiguous E4M3 codes: the hardware conversion of values clamped
+// to 448, which gives e4m3_code's byte for all but NaN.
 template <int W>
 FA_DEV void store_codes(uint8_t* out, const float (&f)[W]) {
   if constexpr (W == 1) {
     out[0] = f32_to_e4m3(f[0]);
   } else {
     uint32_t w[W / 4];
+    bool nan = false;
 #pragma unroll
-    for (int j = 0; j < W; ++j) {
-      const uint32_t code = e4m3_code(f[j]) & 0xffu;
-      if (j % 4 == 0) w[j / 4] = code;
-      else w[j / 4] |= code << (8 * (j % 4));
+    for (int j = 0; j < W; j += 4) {
+      float x[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        x[k] = __builtin_amdgcn_fmed3f(f[j + k], -448.0f, 448.0f);
+        nan |= f[j + k] != f[j + k];
+      }
+      const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+      w[j / 4] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], lo, true);
+    }
+    if (__builtin_expect(nan, 0)) {
+#pragma unroll
+      for (int j = 0; j < W; ++j)
+        if (f[j] != f[j]) w[j / 4] = (w[j / 4] & ~(0xffu << (8 * (j % 4)))) | (e4m3_code(f[j]) & 0xffu) << (8 * (j % 4));
     }
     if constexpr (W == 8) *(uint2*)out = make_uint2(w[0], w[1]);
     else *(uint32_t*)out = w[0];
   }
 }
 
+template <int W>
+FA_DEV void load_codes(const uint8_t* in, float (&f)[W]) {
+  if constexpr (W == 1) {
+    f[0] = e4m3_to_f32(in[0]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < W; j += 4) {
+      const uint32_t w = *(const uint32_t*)(in + j);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) f[j + k] = e4m3_to_f32(w >> (8 * k) & 0xffu);
+    }
+  }
+}
+
 // ------------------------------------------------------------ rows of a token
 
+// Passes of a wave over a token's rows whose loads are all issued before the
+// first of them is used.
+constexpr int BATCH = 2;
+
 template <typename XT, int CACHE, int W>
-FA_DEV void token_rows(const AppendParams& p, int64_t t, int wave, int lane) {
+FA_DEV void token_rows(const AppendParams& p, uint32_t w, int lane) {
   const bool keeps = CACHE == CACHE_SAME || CACHE == CACHE_E4M3;   // k and v of this token go to the cache as rows
+  const int64_t t = w / p.token_waves;
+  if (t >= p.tokens) return;
+  const int per = 64 / p.lanes, sub = lane / p.lanes;
+  const int total = p.passes[0] + p.passes[1] + p.passes[2];
+  const bool inter = p.rot.interleaved;
   int b = -1;
-  int64_t pos = -1, page = -1;
+  int64_t pos = -1;
+  Place at{-1, 0};
   if (CACHE != CACHE_NONE && (keeps || !p.rot.positions)) {
-    b = last_at_most(p.batch + 1, t, lane, [&](int i) { return cu_at(p, i); });
+    b = last_at_most(p.batch + 1, t, lane, [&](int i) { return (int64_t)cu_at(p, i); });
     if (b >= p.batch) b = -1;
     if (b >= 0) {
-      pos = (int64_t)p.used[b * p.used_stride] - cu_at(p, b + 1) + t;
-      if (keeps) page = page_of(p, b, pos);
+      pos = (int64_t)load_invariant_i32(p.used, b * p.used_stride) - cu_of(p, b + 1) + t;
+      if (keeps) at = place_of(p, b, pos);
     }
   }
   const bool q_turns = CACHE == CACHE_NONE || p.rot.positions || b >= 0;
-  const bool inter = p.rot.interleaved;
-  const int per = 64 / p.lanes;   // heads of a wave at once
-  if (lane >= per * p.lanes) return;
-  for (int u = lane % p.lanes; u < 256; u += p.lanes) {
-    if (u >= max(max(p.part[0].units, p.part[1].units), p.part[2].units)) break;
+  for (int u = lane % p.lanes; u < 256; u += 64) {   // (one round but for pieces of one element)
     float c[W], s[W];
     bool have = false;
-    for (int g = wave * per + lane / p.lanes; g < p.row_heads; g += WAVES * per) {
-      int h = g, which = 0;
-      if (h >= p.part[0].heads) h -= p.part[0].heads, which = 1;
-      if (which == 1 && h >= p.part[1].heads) h -= p.part[1].heads, which = 2;
-      const AppendRows& r = p.part[which];
-      if (u >= r.units) continue;
-      const bool cached = CACHE != CACHE_NONE && which > 0;
-      if (cached && page < 0) continue;
-      int lo, hi;
-      bool turns;
-      unit_places<W>(r, inter, u, lo, hi, turns);
-      const int64_t src = t * r.xs[0] + h * r.xs[1];
-      const Piece<XT, W> a = load_piece<XT, W>(r.x, src + lo * r.xs[2], r.xs[2]);
-      Piece<XT, W> z = a;
-      if (hi >= 0) z = load_piece<XT, W>(r.x, src + hi * r.xs[2], r.xs[2]);
-      turns = turns && (cached || q_turns);
-      if (turns && !have) {
+    for (int s0 = (int)(w % p.token_waves); s0 < total; s0 += BATCH * (int)p.token_waves) {
+      Piece<W> a[BATCH], z[BATCH];
+      bool on[BATCH];
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k) {
+        const int pass = s0 + k * (int)p.token_waves;
+        const int which = pass < p.passes[0] ? 0 : pass < p.passes[0] + p.passes[1] ? 1 : 2;
+        const int h = (pass - (which > 0 ? p.passes[0] : 0) - (which > 1 ? p.passes[1] : 0)) * per + sub;
+        const AppendRows& r = p.part[which];
+        on[k] = pass < total && sub < per && h < r.heads && u < r.units && (CACHE == CACHE_NONE || which == 0 || at.page >= 0);
+        if (!on[k]) continue;
+        const Unit x = unit_of<W>(r, inter, u);
+        const int64_t src = t * r.xs[0] + h * r.xs[1];
+        a[k] = load_piece<XT, W>(r.x, src + x.lo * r.xs[2]);
+        z[k] = x.hi >= 0 ? load_piece<XT, W>(r.x, src + x.hi * r.xs[2]) : a[k];
+      }
+      // (Parts that do not turn come last, so a batch that turns starts with one that does.)
+      if (!have && u * W < p.part[s0 < p.passes[0] ? 0 : 1].half && s0 < p.passes[0] + p.passes[1]) {
         load_trig<W>(p, t, pos, u * W, c, s);
         have = true;
       }
-      const int64_t row = cached ? pos % p.page_size : t;
-      const int64_t dst = (cached ? page : 0) * r.os[0] + row * r.os[1] + h * r.os[2];
-      const bool codes = CACHE == CACHE_E4M3 && cached;
-      if (!turns && !codes) {
-        store_piece<XT, W>(r.out, dst + lo * r.os[3], a);
-        if (hi >= 0) store_piece<XT, W>(r.out, dst + hi * r.os[3], z);
-        continue;
-      }
-      float x[W], y[W];
-      widen<XT, W>(a, x);
-      widen<XT, W>(z, y);
-      if (turns) turn<W>(x, y, c, s, inter);
-      if (codes) {
-        const float scale = r.scale[h * r.scale_stride];
 #pragma unroll
-        for (int j = 0; j < W; ++j) x[j] /= scale, y[j] /= scale;
-        store_codes<W>((uint8_t*)r.out + dst + lo * r.os[3], x);
-        if (hi >= 0) store_codes<W>((uint8_t*)r.out + dst + hi * r.os[3], y);
-      } else {
-        store_piece<XT, W>(r.out, dst + lo * r.os[3], narrow<XT, W>(x));
-        if (hi >= 0) store_piece<XT, W>(r.out, dst + hi * r.os[3], narrow<XT, W>(y));
+      for (int k = 0; k < BATCH; ++k) {
+        if (!on[k]) continue;
+        const int pass = s0 + k * (int)p.token_waves;
+        const int which = pass < p.passes[0] ? 0 : pass < p.passes[0] + p.passes[1] ? 1 : 2;
+        const int h = (pass - (which > 0 ? p.passes[0] : 0) - (which > 1 ? p.passes[1] : 0)) * per + sub;
+        const AppendRows& r = p.part[which];
+        const Unit x = unit_of<W>(r, inter, u);
+        const bool cached = CACHE != CACHE_NONE && which > 0;
+        const bool turns = x.turns && (cached || q_turns);
+        const int64_t dst = (cached ? at.page * r.os[0] + at.row * r.os[1] : t * r.os[1]) + h * r.os[2];
+        const bool codes = CACHE == CACHE_E4M3 && cached;
+        if (!turns && !codes) {
+          store_piece<XT, W>(r.out, dst + x.lo * r.os[3], a[k]);
+          if (x.hi >= 0) store_piece<XT, W>(r.out, dst + x.hi * r.os[3], z[k]);
+          continue;
+        }
+        float f[W], g[W];
+        widen<XT, W>(a[k], f);
+        widen<XT, W>(z[k], g);
+        if (turns) turn<W>(f, g, c, s, inter);
+        if (codes) {
+          const float scale = r.scale[h * r.scale_stride];
+#pragma unroll
+          for (int j = 0; j < W; ++j) f[j] /= scale, g[j] /= scale;
+          store_codes<W>((uint8_t*)r.out + dst + x.lo * r.os[3], f);
+          if (x.hi >= 0) store_codes<W>((uint8_t*)r.out + dst + x.hi * r.os[3], g);
+        } else {
+          store_piece<XT, W>(r.out, dst + x.lo * r.os[3], narrow<XT, W>(f));
+          if (x.hi >= 0) store_piece<XT, W>(r.out, dst + x.hi * r.os[3], narrow<XT, W>(g));
+        }
       }
     }
+    if (u + 64 >= 256 || p.lanes < 64) break;
   }
 }
 
@@ -274,111 +414,167 @@ FA_DEV int block_exponent(float most) {
   return max(e, -100);
 }
 
-// x * 2^-e, exact (e in -127 .. 127, any fp32 x whose result E4M3 tells from zero).
-FA_DEV float unscale(float x, int e) { return ldexpf(x, -e); }
+// Rows a lane holds between a block's two passes: with 16 lanes a row (256-dim
+// heads) 32 tokens, with 8 lanes 64, in 64 registers.
+constexpr int HOLD = 8;
 
 template <typename XT, int W>
 FA_DEV void own_block(const AppendParams& p, uint32_t w, int lane) {
-  const int heads = p.part[1].heads;
-  const int h = (int)(w % (uint32_t)heads), which = (int)(w / (uint32_t)heads) & 1;
-  const int64_t id = w / (2u * (uint32_t)heads);
-  const int64_t block = p.block;
+  const uint32_t heads = (uint32_t)p.part[1].heads;
+  const int h = (int)(w % heads), which = (int)(w / heads) & 1;
+  const int id = (int)(w / (2 * heads)), block = p.block;
   // A request of n rows touches at most n / block + 2 blocks: request b has the
   // ids from cu[b] / block + 2 b on.
-  const int b = last_at_most(p.batch, id, lane, [&](int i) { return cu_at(p, i) / block + 2 * i; });
+  const int b = last_at_most(p.batch, id, lane, [&](int i) { return (int64_t)(cu_at(p, i) / block) + 2 * (int64_t)i; });
   if (b < 0) return;
-  const int64_t t0 = cu_at(p, b), n = cu_at(p, b + 1) - t0;
-  const int64_t end = p.used[b * p.used_stride], start = end - n;
+  const int t0 = cu_of(p, b);
+  const int64_t n = (int64_t)cu_of(p, b + 1) - t0;
+  const int64_t end = load_invariant_i32(p.used, b * p.used_stride), start = end - n;
   if (t0 < 0 || n <= 0 || end <= 0) return;
   const int64_t from = max(start, (int64_t)0);
-  const int64_t base = (from / block + (id - t0 / block - 2 * b)) * block;   // the block's first position
+  const int64_t base = ((uint32_t)from / (uint32_t)block + (int64_t)(id - t0 / block - 2 * b)) * block;   // its first position
   if (base >= end || base - start >= p.tokens - t0) return;
-  const int64_t page = page_of(p, b, base);
-  if (page < 0) return;
+  const Place place = place_of(p, b, base);
+  if (place.page < 0) return;
   // The block's new rows (none past the last row there is).
-  const int first = (int)(max(base, from) - base), last = (int)(min(min(base + block, end), start + p.tokens - t0) - base);
+  const int first = (int)(max(base, from) - base);
+  const int last = (int)(min(min(base + block, end), start + p.tokens - t0) - base);
   const AppendRows& r = p.part[1 + which];
-  const int64_t row0 = base % p.page_size;
-  const int64_t x0 = (t0 + base - start) * r.xs[0] + h * r.xs[1];
-  const int64_t o0 = page * r.os[0] + row0 * r.os[1] + h * r.os[2];
+  const int64_t token = t0 + base - start;   // row 0's
+  const void* const x0 = (const typename XT::storage*)r.x + token * r.xs[0] + h * r.xs[1];
+  uint8_t* const o0 = (uint8_t*)r.out + place.page * r.os[0] + place.row * r.os[1] + h * r.os[2];
   const bool inter = p.rot.interleaved;
-  const int per = 64 / p.lanes, rl = lane / p.lanes;
-  const bool on = rl < per;
-  uint8_t* const sp = p.block_scale[which] + page * p.block_stride[which][0] + row0 / block * p.block_stride[which][1] +
-                      h * p.block_stride[which][2];
-  // f(row, lo, hi, values of the pieces) over this lane's units of the new rows.
-  auto each = [&](auto f) {
-    for (int row = first + rl; row < last; row += per) {
-      for (int u = lane % p.lanes; u < r.units; u += p.lanes) {
-        int lo, hi;
-        bool turns;
-        unit_places<W>(r, inter, u, lo, hi, turns);
-        const int64_t src = x0 + row * r.xs[0];
-        float x[W], y[W];
-        widen<XT, W>(load_piece<XT, W>(r.x, src + lo * r.xs[2], r.xs[2]), x);
-        if (hi >= 0) widen<XT, W>(load_piece<XT, W>(r.x, src + hi * r.xs[2], r.xs[2]), y);
-        else
-#pragma unroll
-          for (int j = 0; j < W; ++j) y[j] = 0.0f;
-        if (turns) {
-          float c[W], s[W];
-          load_trig<W>(p, t0 + base + row - start, base + row, u * W, c, s);
-          turn<W>(x, y, c, s, inter);
-        }
-        f(row, lo, hi, x, y);
-      }
+  const int per = 64 / p.lanes, sub = lane / p.lanes;
+  const bool on = sub < per;
+  uint8_t* const sp = p.block_scale[which] + place.page * p.block_stride[which][0] +
+                      (uint32_t)place.row / (uint32_t)block * p.block_stride[which][1] + h * p.block_stride[which][2];
+  const int old = first > 0 ? (int)sp[0] - 127 : 0;
+
+  // The pieces of one unit of a row, as they come and turned.
+  auto load = [&](int row, const Unit& x, Piece<W>& a, Piece<W>& z) {
+    a = load_piece<XT, W>(x0, row * r.xs[0] + x.lo * r.xs[2]);
+    z = x.hi >= 0 ? load_piece<XT, W>(x0, row * r.xs[0] + x.hi * r.xs[2]) : Piece<W>{};
+  };
+  auto turned = [&](int row, int u, const Unit& x, const Piece<W>& a, const Piece<W>& z, float (&f)[W], float (&g)[W]) {
+    widen<XT, W>(a, f);
+    widen<XT, W>(z, g);
+    if (x.turns) {
+      float c[W], s[W];
+      load_trig<W>(p, token + row, base + row, u * W, c, s);
+      turn<W>(f, g, c, s, inter);
     }
   };
-  float most = 0.0f;
-  if (on)
-    each([&](int, int, int, float (&x)[W], float (&y)[W]) {
+  auto largest = [&](float most, const float (&f)[W], const float (&g)[W]) {
 #pragma unroll
-      for (int j = 0; j < W; ++j) {
-        const float a = fabsf(x[j]), z = fabsf(y[j]);
-        most = fmaxf(most, a < INFINITY ? a : 0.0f);
-        most = fmaxf(most, z < INFINITY ? z : 0.0f);
-      }
-    });
-  int e = block_exponent(wave_max(most));
-  if (first > 0) {
-    const int old = (int)sp[0] - 127;
-    if (old >= e) {
-      e = old;
-    } else if (on) {
-      // Rows of the request before the new ones, under the larger scale.
-      for (int row = rl; row < first; row += per) {
+    for (int j = 0; j < W; ++j) {
+      const float a = fabsf(f[j]), z = fabsf(g[j]);
+      most = fmaxf(most, a < INFINITY ? a : 0.0f);
+      most = fmaxf(most, z < INFINITY ? z : 0.0f);
+    }
+    return most;
+  };
+  // The block's scale from its rows' largest magnitude; rows of the request
+  // before the new ones are coded again where it grows.
+  auto settle = [&](float most) {
+    const int e = block_exponent(wave_max(most));
+    if (first == 0) return e;
+    if (old >= e) return old;
+    if (on) {
+      for (int row = sub; row < first; row += per) {
         for (int u = lane % p.lanes; u < r.units; u += p.lanes) {
-          int place[2];
-          bool turns;
-          unit_places<W>(r, inter, u, place[0], place[1], turns);
+          const Unit x = unit_of<W>(r, inter, u);
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            if (place[i] < 0) continue;
-            uint8_t* const at = (uint8_t*)r.out + o0 + row * r.os[1] + place[i] * r.os[3];
+            const int place = i ? x.hi : x.lo;
+            if (place < 0) continue;
+            uint8_t* const at = o0 + row * r.os[1] + place * r.os[3];
             float f[W];
+            load_codes<W>(at, f);
 #pragma unroll
-            for (int j = 0; j < W; ++j) f[j] = unscale(e4m3_to_f32(at[j]), e - old);
+            for (int j = 0; j < W; ++j) f[j] = ldexpf(f[j], old - e);
             store_codes<W>(at, f);
           }
         }
       }
     }
-  }
-  if (on)
-    each([&](int row, int lo, int hi, float (&x)[W], float (&y)[W]) {
+    return e;
+  };
+  auto store = [&](int row, const Unit& x, float (&f)[W], float (&g)[W], float inverse) {
 #pragma unroll
-      for (int j = 0; j < W; ++j) x[j] = unscale(x[j], e), y[j] = unscale(y[j], e);
-      uint8_t* const at = (uint8_t*)r.out + o0 + row * r.os[1];
-      store_codes<W>(at + lo * r.os[3], x);
-      if (hi >= 0) store_codes<W>(at + hi * r.os[3], y);
-    });
+    for (int j = 0; j < W; ++j) f[j] *= inverse, g[j] *= inverse;   // exact where E4M3 tells it from zero
+    uint8_t* const at = o0 + row * r.os[1];
+    store_codes<W>(at + x.lo * r.os[3], f);
+    if (x.hi >= 0) store_codes<W>(at + x.hi * r.os[3], g);
+  };
+  int e;
+  const int count = last - first;
+  if (W > 1 && count <= per) {
+    // One row a lane (a decode step's one): the turned values stay.
+    const int u = lane % p.lanes, row = first + sub;
+    const bool mine = on && u < r.units && sub < count;
+    const Unit x = unit_of<W>(r, inter, u);
+    float f[W], g[W], most = 0.0f;
+    if (mine) {
+      Piece<W> a, z;
+      load(row, x, a, z);
+      turned(row, u, x, a, z, f, g);
+      most = largest(most, f, g);
+    }
+    e = settle(most);
+    if (mine) store(row, x, f, g, ldexpf(1.0f, -e));
+  } else if (W > 1 && count <= HOLD * per) {
+    const int u = lane % p.lanes;
+    const bool mine = on && u < r.units;
+    const Unit x = unit_of<W>(r, inter, u);
+    Piece<W> a[HOLD], z[HOLD];
+#pragma unroll
+    for (int i = 0; i < HOLD; ++i)
+      if (mine && i * per + sub < count) load(first + i * per + sub, x, a[i], z[i]);
+    float most = 0.0f;
+#pragma unroll
+    for (int i = 0; i < HOLD; ++i) {
+      if (!(mine && i * per + sub < count)) continue;
+      float f[W], g[W];
+      turned(first + i * per + sub, u, x, a[i], z[i], f, g);
+      most = largest(most, f, g);
+    }
+    e = settle(most);
+    const float inverse = ldexpf(1.0f, -e);
+#pragma unroll
+    for (int i = 0; i < HOLD; ++i) {
+      if (!(mine && i * per + sub < count)) continue;
+      float f[W], g[W];
+      turned(first + i * per + sub, u, x, a[i], z[i], f, g);
+      store(first + i * per + sub, x, f, g, inverse);
+    }
+  } else {
+    // Long blocks and pieces of one element: the rows are read twice.
+    auto each = [&](auto use) {
+      if (!on) return;
+      for (int row = first + sub; row < last; row += per) {
+        for (int u = lane % p.lanes; u < r.units; u += p.lanes) {
+          const Unit x = unit_of<W>(r, inter, u);
+          Piece<W> a, z;
+          load(row, x, a, z);
+          float f[W], g[W];
+          turned(row, u, x, a, z, f, g);
+          use(row, x, f, g);
+        }
+      }
+    };
+    float most = 0.0f;
+    each([&](int, const Unit&, float (&f)[W], float (&g)[W]) { most = largest(most, f, g); });
+    e = settle(most);
+    const float inverse = ldexpf(1.0f, -e);
+    each([&](int row, const Unit& x, float (&f)[W], float (&g)[W]) { store(row, x, f, g, inverse); });
+  }
   if (lane == 0) sp[0] = (uint8_t)(e + 127);
 }
 
 template <typename XT, int CACHE, int W>
 __global__ __launch_bounds__(THREADS) void append_kernel(const AppendParams p) {
   const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   uint32_t group = blockIdx.x;
   if constexpr (CACHE == CACHE_BLOCK) {
     const uint32_t groups = (p.block_waves + WAVES - 1) / WAVES;
@@ -389,7 +585,7 @@ __global__ __launch_bounds__(THREADS) void append_kernel(const AppendParams p) {
     }
     group -= groups;
   }
-  token_rows<XT, CACHE, W>(p, group, wave, lane);
+  token_rows<XT, CACHE, W>(p, group * WAVES + wave, lane);
 }
 
 // ------------------------------------------------------------ host
@@ -448,6 +644,13 @@ bool pieces_aligned(const AppendRows& p, int esz, int osz) {
   return true;
 }
 
+// Whether cos and sin come in aligned pieces wherever a unit's start in their rows.
+bool trig_aligned(const fa_rotation& r) {
+  const int esz = r.trig_dtype == FA_F32 ? 4 : 2;
+  return r.cos_stride[1] == 1 && r.sin_stride[1] == 1 && (uintptr_t)r.cos_table % 16 == 0 &&
+         (uintptr_t)r.sin_table % 16 == 0 && (r.cos_stride[0] * esz) % 16 == 0 && (r.sin_stride[0] * esz) % 16 == 0;
+}
+
 template <typename XT, int W>
 void launch_append(int cache, const AppendParams& p, uint32_t groups, hipStream_t s) {
   const dim3 grid(groups), block(THREADS);
@@ -462,7 +665,7 @@ void launch_append(int cache, const AppendParams& p, uint32_t groups, hipStream_
 // Fills in what the parts have in common and launches.
 int run_append(AppendParams& p, int dtype, int cache, void* stream, const char* who) {
   const int esz = dtype == FA_F32 ? 4 : 2;
-  bool vec = true;
+  bool vec = !p.rot.cos_table || trig_aligned(p.rot);
   for (int i = 0; i < 3; ++i) {
     AppendRows& r = p.part[i];
     const bool cached = cache != CACHE_NONE && i > 0;
@@ -477,11 +680,20 @@ int run_append(AppendParams& p, int dtype, int cache, void* stream, const char* 
     units = r.units > units ? r.units : units;
   }
   p.lanes = units < 64 ? units : 64;
-  p.row_heads = p.part[0].heads + (cache == CACHE_BLOCK ? 0 : p.part[1].heads + p.part[2].heads);
-  int64_t groups = p.row_heads ? p.tokens : 0;
+  int64_t passes = 0;
+  for (int i = 0; i < 3; ++i) {
+    p.passes[i] = cache == CACHE_BLOCK && i > 0 ? 0 : (int)fa_ceil_div(p.part[i].heads, 64 / p.lanes);
+    passes += p.passes[i];
+  }
+  // A few tokens: every pass over a token's rows on a wave of its own, for the
+  // shortest chain.  Many: BATCH passes a wave, which finds its request, position
+  // and cos/sin once for them.
+  p.token_waves = (uint32_t)(passes == 0 ? 1 : p.tokens * passes <= 4096 ? passes : fa_ceil_div(passes, BATCH));
+  int64_t groups = passes ? fa_ceil_div(p.tokens * p.token_waves, WAVES) : 0;
+  FA_REQUIRE(p.tokens * p.token_waves <= INT32_MAX, "%s: too many rows", who);
   if (cache == CACHE_BLOCK) {
     const int64_t waves = (p.tokens / p.block + 2 * (int64_t)p.batch) * 2 * p.part[1].heads;
-    FA_REQUIRE(waves <= 0x7fffffffll, "%s: too many blocks", who);
+    FA_REQUIRE(waves <= INT32_MAX, "%s: too many blocks", who);
     p.block_waves = (uint32_t)waves;
     groups += fa_ceil_div(waves, WAVES);
   }
@@ -558,7 +770,8 @@ extern "C" int fa_paged_append(const fa_paged_append_args* a, void* stream) {
   p.used = a->seqused_k, p.used_stride = a->used_k_stride;
   p.table = a->block_table;
   for (int i = 0; i < 2; ++i) p.bt_stride[i] = a->bt_stride[i];
-  p.tokens = a->tokens, p.batch = (int32_t)a->batch, p.page_size = a->page_size;
+  p.tokens = a->tokens, p.batch = (int32_t)a->batch;
+  p.page_size = (int32_t)(a->page_size < INT32_MAX ? a->page_size : INT32_MAX);
   p.num_pages = a->num_pages, p.table_cols = a->table_cols;
   p.block = (int32_t)a->block;
   return run_append(p, xdt, a->block ? CACHE_BLOCK : cdt == FA_E4M3 ? CACHE_E4M3 : CACHE_SAME, stream, who);
