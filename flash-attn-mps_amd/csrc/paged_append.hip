@@ -17,15 +17,17 @@
 // works on one token, or on one block of one head: what follows from those
 // (request, position, page) is scalar.
 //
-// Block-scaled caches: one wave owns a (block of tokens, head) of K or V, so
-// the block's largest magnitude, its scale and its rows need no other wave, and
-// the result does not depend on any order.  The rows stay in registers between
-// the two passes that this takes, up to HOLD rows a lane.
+// Block-scaled caches: a workgroup owns a block of tokens of as many heads of K or
+// V as a wave holds of a row, its waves the rows in turn, so a block's largest
+// magnitude (a maximum in LDS), its scale and its rows need no one else, and the
+// result does not depend on any order.  The rows stay in registers until the scale
+// is known, and are turned a second time (16 registers a row would hold them
+// turned, 8 do as they came).
 #include "attn_common.h"
 
 namespace {
 
-constexpr int THREADS = 256, WAVES = 4;
+constexpr int THREADS = 256, MOST_THREADS = 1024;
 
 // What an append writes: nothing, rows of the input's type, E4M3 with a scale
 // per head, E4M3 with a scale per block.
@@ -49,10 +51,13 @@ struct AppendParams {
   int64_t cu_stride, used_stride, bt_stride[2];
   int64_t tokens, num_pages, table_cols;
   int32_t batch, page_size, block;   // page_size: clipped to 32 bits, as positions are
-  int32_t lanes;                     // units of a row handled at once
+  int32_t lanes, per;                // units of a row handled at once, rows (64 / lanes)
+  uint32_t lane_part;                // 2^16 / lanes, rounded up: lane / lanes = lane * lane_part >> 16
   int32_t passes[3];                 // passes of 64 / lanes heads over each part's rows (0: not as rows)
   uint32_t token_waves;              // waves of a token
-  uint32_t block_waves;              // workgroups 0 .. ceil(block_waves / 4) - 1 own blocks
+  int32_t head_sets;                 // sets of `per` heads
+  uint32_t block_groups;             // workgroups that own blocks, before those of the tokens
+  uint32_t threads;
 };
 
 // The largest i < n with key(i) <= target (key nondecreasing), -1 if none: 64
@@ -104,59 +109,85 @@ FA_DEV int64_t position_of(const AppendParams& p, int64_t t, int axis) {
   return p.rot.position_dtype == FA_I64 ? ((const int64_t*)p.rot.positions)[at] : ((const int32_t*)p.rot.positions)[at];
 }
 
+// W elements as they are stored: 16 bytes, or one element's bits.
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+template <int W> struct PieceOf { using type = u32x4; };
+template <> struct PieceOf<1> { using type = uint32_t; };
+template <int W> using Piece = typename PieceOf<W>::type;
+
+template <int BYTES> struct LoadOf { using type = u32x4; };
+template <> struct LoadOf<8> { using type = u32x2; };
+
+template <typename XT>
+FA_DEV float value_of_bits(uint32_t bits) {
+  if constexpr (XT::id == FA_F32) return __uint_as_float(bits);
+  else if constexpr (XT::id == FA_BF16) return bf16_bits_to_f32(bits);
+  else return f16_bits_to_f32(bits);
+}
+
+// Element j of a vector of T.
+template <typename T, typename V>
+FA_DEV float value_at(V v, int j) {
+  return value_of_bits<T>(T::bytes == 4 ? v[j] : v[j / 2] >> (16 * (j & 1)) & 0xffffu);
+}
+
+// What a position without a table row reads: NaN in every type.
+#define FA_NAN4 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u
+#define FA_NAN32 FA_NAN4, FA_NAN4, FA_NAN4, FA_NAN4, FA_NAN4, FA_NAN4, FA_NAN4, FA_NAN4
+static __device__ const __align__(16) uint32_t nan_row[256] = {FA_NAN32, FA_NAN32, FA_NAN32, FA_NAN32,
+                                                               FA_NAN32, FA_NAN32, FA_NAN32, FA_NAN32};
+
 // cos and sin of pairs i .. i + W - 1 at row `row` of the tables (W > 1: aligned
-// pieces of contiguous rows); NaN without one.
-template <int W>
+// pieces of contiguous rows of TT).  Without a branch, so that the loads of
+// several rows are in flight together.
+template <typename TT, int W>
 FA_DEV void load_row(const AppendParams& p, int64_t row, int i, float (&c)[W], float (&s)[W]) {
-#pragma unroll
-  for (int j = 0; j < W; ++j) c[j] = s[j] = __builtin_nanf("");
-  if (row < 0 || row >= p.rot.table_rows) return;
-  const int64_t ca = row * p.rot.cos_stride[0], sa = row * p.rot.sin_stride[0];
+  const bool in = row >= 0 && row < p.rot.table_rows;
   if constexpr (W == 1) {
-    c[0] = load_any(p.rot.cos_table, ca + i * p.rot.cos_stride[1], p.rot.trig_dtype);
-    s[0] = load_any(p.rot.sin_table, sa + i * p.rot.sin_stride[1], p.rot.trig_dtype);
-  } else if (p.rot.trig_dtype == FA_F32) {
-#pragma unroll
-    for (int j = 0; j < W; j += 4) {
-      const float4 x = *(const float4*)((const float*)p.rot.cos_table + ca + i + j);
-      const float4 y = *(const float4*)((const float*)p.rot.sin_table + sa + i + j);
-      c[j] = x.x, c[j + 1] = x.y, c[j + 2] = x.z, c[j + 3] = x.w;
-      s[j] = y.x, s[j + 1] = y.y, s[j + 2] = y.z, s[j + 3] = y.w;
-    }
+    c[0] = s[0] = __builtin_nanf("");
+    if (!in) return;
+    c[0] = load_any(p.rot.cos_table, row * p.rot.cos_stride[0] + i * p.rot.cos_stride[1], p.rot.trig_dtype);
+    s[0] = load_any(p.rot.sin_table, row * p.rot.sin_stride[0] + i * p.rot.sin_stride[1], p.rot.trig_dtype);
   } else {
-    const bool bf = p.rot.trig_dtype == FA_BF16;
+    using S = typename TT::storage;
+    const S* const ct = in ? (const S*)p.rot.cos_table + row * p.rot.cos_stride[0] : (const S*)nan_row;
+    const S* const st = in ? (const S*)p.rot.sin_table + row * p.rot.sin_stride[0] : (const S*)nan_row;
+    constexpr int N = 16 / TT::bytes < W ? 16 / TT::bytes : W;   // values of a load
+    using V = typename LoadOf<N * TT::bytes>::type;
 #pragma unroll
-    for (int j = 0; j < W; j += 4) {
-      const uint2 x = *(const uint2*)((const uint16_t*)p.rot.cos_table + ca + i + j);
-      const uint2 y = *(const uint2*)((const uint16_t*)p.rot.sin_table + sa + i + j);
+    for (int j = 0; j < W; j += N) {
+      const V x = *(const V*)(ct + (uint32_t)(i + j)), y = *(const V*)(st + (uint32_t)(i + j));
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint32_t u = (k & 2 ? x.y : x.x) >> (16 * (k & 1)) & 0xffffu, v = (k & 2 ? y.y : y.x) >> (16 * (k & 1)) & 0xffffu;
-        c[j + k] = bf ? bf16_bits_to_f32(u) : f16_bits_to_f32(u);
-        s[j + k] = bf ? bf16_bits_to_f32(v) : f16_bits_to_f32(v);
+      for (int k = 0; k < N; ++k) {
+        c[j + k] = value_at<TT>(x, k);
+        s[j + k] = value_at<TT>(y, k);
       }
     }
   }
 }
 
-// cos and sin of pairs i .. i + W - 1 (i a multiple of W) of token t: a row for
-// each axis that they have, which is one unless axes alternate.
-template <int W>
+// cos and sin of pairs i .. i + W - 1 (i a multiple of W) of token t: at its
+// cache position, or (POS) at the positions of the pairs' axes.
+template <typename TT, bool POS, int W>
 FA_DEV void load_trig(const AppendParams& p, int64_t t, int64_t cache_pos, int i, float (&c)[W], float (&s)[W]) {
-  const uint32_t axes = p.rot.positions ? pair_axes(p, i) : 0;
-  uint32_t todo = 0;
+  if constexpr (!POS) {
+    load_row<TT, W>(p, cache_pos, i, c, s);
+  } else {
+    constexpr uint32_t MASK = (1u << (2 * W)) - 1, ONES = MASK / 3;
+    const uint32_t axes = p.rot.axes > 1 ? pair_axes(p, i) & MASK : 0;
+    load_row<TT, W>(p, position_of(p, t, axes & 3), i, c, s);
+    if (W == 1 || axes == (axes & 3) * ONES) return;
+    // Axes that alternate within a unit: the others' rows.
+    for (uint32_t axis = 0; axis < (uint32_t)p.rot.axes; ++axis) {
+      float ca[W], sa[W];
+      load_row<TT, W>(p, position_of(p, t, axis), i, ca, sa);
 #pragma unroll
-  for (int j = 0; j < W; ++j) todo |= 1u << (axes >> (2 * j) & 3);
-  while (todo) {
-    const uint32_t axis = (uint32_t)__builtin_ctz(todo);
-    todo &= todo - 1;
-    float ca[W], sa[W];
-    load_row<W>(p, p.rot.positions ? position_of(p, t, axis) : cache_pos, i, ca, sa);
-#pragma unroll
-    for (int j = 0; j < W; ++j) {
-      const bool own = (axes >> (2 * j) & 3) == axis;
-      c[j] = own ? ca[j] : c[j];
-      s[j] = own ? sa[j] : s[j];
+      for (int j = 0; j < W; ++j) {
+        const bool own = (axes >> (2 * j) & 3) == axis;
+        c[j] = own ? ca[j] : c[j];
+        s[j] = own ? sa[j] : s[j];
+      }
     }
   }
 }
@@ -183,12 +214,6 @@ FA_DEV Unit unit_of(const AppendRows& r, bool interleaved, int u) {
   return x;
 }
 
-// W elements as they are stored: 16 bytes, or one element's bits.
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-template <int W> struct PieceOf { using type = u32x4; };
-template <> struct PieceOf<1> { using type = uint32_t; };
-template <int W> using Piece = typename PieceOf<W>::type;
-
 template <typename XT, int W>
 FA_DEV Piece<W> load_piece(const void* x, int64_t at) {
   using S = typename XT::storage;
@@ -210,18 +235,14 @@ FA_DEV void store_piece(void* x, int64_t at, Piece<W> v) {
   else ((S*)x)[at] = (S)v;
 }
 
-template <typename XT>
-FA_DEV float value_of_bits(uint32_t bits) {
-  if constexpr (XT::id == FA_F32) return __uint_as_float(bits);
-  else if constexpr (XT::id == FA_BF16) return bf16_bits_to_f32(bits);
-  else return f16_bits_to_f32(bits);
-}
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
 
+// Two values rounded to XT's 16 bits, in one word.
 template <typename XT>
-FA_DEV uint32_t bits_of_value(float f) {
-  if constexpr (XT::id == FA_F32) return __float_as_uint(f);
-  else if constexpr (XT::id == FA_BF16) return f32_to_bf16_bits(f);
-  else return f32_to_f16_bits(f);
+FA_DEV uint32_t pack2(float lo, float hi) {
+  if constexpr (XT::id == FA_BF16) return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)lo, (__bf16)hi});
+  else return __builtin_bit_cast(uint32_t, f16x2{(_Float16)lo, (_Float16)hi});
 }
 
 template <typename XT, int W>
@@ -230,21 +251,18 @@ FA_DEV void widen(Piece<W> v, float (&f)[W]) {
     f[0] = value_of_bits<XT>(v);
   } else {
 #pragma unroll
-    for (int j = 0; j < W; ++j)
-      f[j] = value_of_bits<XT>(XT::bytes == 4 ? v[j % 4] : v[j / 2] >> (16 * (j & 1)) & 0xffffu);
+    for (int j = 0; j < W; ++j) f[j] = value_at<XT>(v, j);
   }
 }
 
 template <typename XT, int W>
 FA_DEV Piece<W> narrow(const float (&f)[W]) {
   if constexpr (W == 1) {
-    return bits_of_value<XT>(f[0]);
+    return XT::bytes == 4 ? __float_as_uint(f[0]) : pack2<XT>(f[0], 0.0f) & 0xffffu;
   } else {
     u32x4 v;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      v[j] = XT::bytes == 4 ? bits_of_value<XT>(f[j % W])
-                            : bits_of_value<XT>(f[2 * j % W]) | bits_of_value<XT>(f[(2 * j + 1) % W]) << 16;
+    for (int j = 0; j < 4; ++j) v[j] = XT::bytes == 4 ? __float_as_uint(f[j % W]) : pack2<XT>(f[2 * j % W], f[(2 * j + 1) % W]);
     return v;
   }
 }
@@ -318,22 +336,37 @@ FA_DEV void load_codes(const uint8_t* in, float (&f)[W]) {
 
 // ------------------------------------------------------------ rows of a token
 
+// A lane's offset of element e of head h within a row: 32 bits for vectors (the
+// host checks that a row fits), 64 for single elements.
+template <int W>
+FA_DEV auto lane_offset(int h, int64_t head_stride, int e, int64_t stride) {
+  if constexpr (W > 1) return (uint32_t)h * (uint32_t)head_stride + (uint32_t)e;
+  else return h * head_stride + e * stride;
+}
+
 // Passes of a wave over a token's rows whose loads are all issued before the
 // first of them is used.
-constexpr int BATCH = 2;
+#ifndef PA_BATCH
+#define PA_BATCH 2
+#endif
+#ifndef PA_MIN
+#define PA_MIN 1
+#endif
+constexpr int BATCH = PA_BATCH;
 
-template <typename XT, int CACHE, int W>
+template <typename XT, typename TT, int CACHE, bool POS, int W>
 FA_DEV void token_rows(const AppendParams& p, uint32_t w, int lane) {
   const bool keeps = CACHE == CACHE_SAME || CACHE == CACHE_E4M3;   // k and v of this token go to the cache as rows
-  const int64_t t = w / p.token_waves;
+  const int64_t t = p.token_waves == 1 ? w : w / p.token_waves;
   if (t >= p.tokens) return;
-  const int per = 64 / p.lanes, sub = lane / p.lanes;
+  const int per = p.per, sub = (int)(lane * p.lane_part >> 16), u0 = lane - sub * p.lanes;
+  const int pass0 = (int)(w - (uint32_t)t * p.token_waves);
   const int total = p.passes[0] + p.passes[1] + p.passes[2];
   const bool inter = p.rot.interleaved;
   int b = -1;
   int64_t pos = -1;
   Place at{-1, 0};
-  if (CACHE != CACHE_NONE && (keeps || !p.rot.positions)) {
+  if (CACHE != CACHE_NONE && (keeps || !POS)) {
     b = last_at_most(p.batch + 1, t, lane, [&](int i) { return (int64_t)cu_at(p, i); });
     if (b >= p.batch) b = -1;
     if (b >= 0) {
@@ -341,11 +374,11 @@ FA_DEV void token_rows(const AppendParams& p, uint32_t w, int lane) {
       if (keeps) at = place_of(p, b, pos);
     }
   }
-  const bool q_turns = CACHE == CACHE_NONE || p.rot.positions || b >= 0;
-  for (int u = lane % p.lanes; u < 256; u += 64) {   // (one round but for pieces of one element)
+  const bool q_turns = CACHE == CACHE_NONE || POS || b >= 0;
+  for (int u = u0; u < 256; u += 64) {   // (one round but for pieces of one element)
     float c[W], s[W];
     bool have = false;
-    for (int s0 = (int)(w % p.token_waves); s0 < total; s0 += BATCH * (int)p.token_waves) {
+    for (int s0 = pass0; s0 < total; s0 += BATCH * (int)p.token_waves) {
       Piece<W> a[BATCH], z[BATCH];
       bool on[BATCH];
 #pragma unroll
@@ -357,13 +390,13 @@ FA_DEV void token_rows(const AppendParams& p, uint32_t w, int lane) {
         on[k] = pass < total && sub < per && h < r.heads && u < r.units && (CACHE == CACHE_NONE || which == 0 || at.page >= 0);
         if (!on[k]) continue;
         const Unit x = unit_of<W>(r, inter, u);
-        const int64_t src = t * r.xs[0] + h * r.xs[1];
-        a[k] = load_piece<XT, W>(r.x, src + x.lo * r.xs[2]);
-        z[k] = x.hi >= 0 ? load_piece<XT, W>(r.x, src + x.hi * r.xs[2]) : a[k];
+        const void* const src = (const typename XT::storage*)r.x + t * r.xs[0];
+        a[k] = load_piece<XT, W>(src, lane_offset<W>(h, r.xs[1], x.lo, r.xs[2]));
+        z[k] = x.hi >= 0 ? load_piece<XT, W>(src, lane_offset<W>(h, r.xs[1], x.hi, r.xs[2])) : a[k];
       }
       // (Parts that do not turn come last, so a batch that turns starts with one that does.)
       if (!have && u * W < p.part[s0 < p.passes[0] ? 0 : 1].half && s0 < p.passes[0] + p.passes[1]) {
-        load_trig<W>(p, t, pos, u * W, c, s);
+        load_trig<TT, POS, W>(p, t, pos, u * W, c, s);
         have = true;
       }
 #pragma unroll
@@ -376,11 +409,13 @@ FA_DEV void token_rows(const AppendParams& p, uint32_t w, int lane) {
         const Unit x = unit_of<W>(r, inter, u);
         const bool cached = CACHE != CACHE_NONE && which > 0;
         const bool turns = x.turns && (cached || q_turns);
-        const int64_t dst = (cached ? at.page * r.os[0] + at.row * r.os[1] : t * r.os[1]) + h * r.os[2];
+        const int64_t dst = cached ? at.page * r.os[0] + at.row * r.os[1] : t * r.os[1];
+        const auto lo = lane_offset<W>(h, r.os[2], x.lo, r.os[3]), hi = lane_offset<W>(h, r.os[2], x.hi, r.os[3]);
         const bool codes = CACHE == CACHE_E4M3 && cached;
+        void* const out = (typename XT::storage*)r.out + (codes ? 0 : dst);
         if (!turns && !codes) {
-          store_piece<XT, W>(r.out, dst + x.lo * r.os[3], a[k]);
-          if (x.hi >= 0) store_piece<XT, W>(r.out, dst + x.hi * r.os[3], z[k]);
+          store_piece<XT, W>(out, lo, a[k]);
+          if (x.hi >= 0) store_piece<XT, W>(out, hi, z[k]);
           continue;
         }
         float f[W], g[W];
@@ -391,11 +426,11 @@ FA_DEV void token_rows(const AppendParams& p, uint32_t w, int lane) {
           const float scale = r.scale[h * r.scale_stride];
 #pragma unroll
           for (int j = 0; j < W; ++j) f[j] /= scale, g[j] /= scale;
-          store_codes<W>((uint8_t*)r.out + dst + x.lo * r.os[3], f);
-          if (x.hi >= 0) store_codes<W>((uint8_t*)r.out + dst + x.hi * r.os[3], g);
+          store_codes<W>((uint8_t*)r.out + dst + lo, f);
+          if (x.hi >= 0) store_codes<W>((uint8_t*)r.out + dst + hi, g);
         } else {
-          store_piece<XT, W>(r.out, dst + x.lo * r.os[3], narrow<XT, W>(f));
-          if (x.hi >= 0) store_piece<XT, W>(r.out, dst + x.hi * r.os[3], narrow<XT, W>(g));
+          store_piece<XT, W>(out, lo, narrow<XT, W>(f));
+          if (x.hi >= 0) store_piece<XT, W>(out, hi, narrow<XT, W>(g));
         }
       }
     }
@@ -414,55 +449,54 @@ FA_DEV int block_exponent(float most) {
   return max(e, -100);
 }
 
-// Rows a lane holds between a block's two passes: with 16 lanes a row (256-dim
-// heads) 32 tokens, with 8 lanes 64, in 64 registers.
-constexpr int HOLD = 8;
+// Rows a lane holds between a block's largest magnitude and its codes.
+constexpr int HOLD = 4;
 
-template <typename XT, int W>
-FA_DEV void own_block(const AppendParams& p, uint32_t w, int lane) {
-  const uint32_t heads = (uint32_t)p.part[1].heads;
-  const int h = (int)(w % heads), which = (int)(w / heads) & 1;
-  const int id = (int)(w / (2 * heads)), block = p.block;
+template <typename XT, typename TT, bool POS, int W>
+FA_DEV void own_block(const AppendParams& p, uint32_t group, int lane, uint32_t* most_of) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = (int)blockDim.x >> 6;
+  const int per = p.per, sub = (int)(lane * p.lane_part >> 16), u0 = lane - sub * p.lanes;
+  const uint32_t heads = (uint32_t)p.part[1].heads, sets = (uint32_t)p.head_sets;
+  const int h = (int)(group % sets) * per + sub, which = (int)(group / sets) & 1;
+  const int id = (int)(group / (2 * sets)), block = p.block;
   // A request of n rows touches at most n / block + 2 blocks: request b has the
   // ids from cu[b] / block + 2 b on.
   const int b = last_at_most(p.batch, id, lane, [&](int i) { return (int64_t)(cu_at(p, i) / block) + 2 * (int64_t)i; });
   if (b < 0) return;
   const int t0 = cu_of(p, b);
   const int64_t n = (int64_t)cu_of(p, b + 1) - t0;
-  const int64_t end = load_invariant_i32(p.used, b * p.used_stride), start = end - n;
+  const int64_t end = load_invariant_i32(p.used, b * p.used_stride), start = end - n, from = max(start, (int64_t)0);
   if (t0 < 0 || n <= 0 || end <= 0) return;
-  const int64_t from = max(start, (int64_t)0);
   const int64_t base = ((uint32_t)from / (uint32_t)block + (int64_t)(id - t0 / block - 2 * b)) * block;   // its first position
   if (base >= end || base - start >= p.tokens - t0) return;
   const Place place = place_of(p, b, base);
-  if (place.page < 0) return;
+  if (place.page < 0) return;   // (so far the same for the whole workgroup)
   // The block's new rows (none past the last row there is).
   const int first = (int)(max(base, from) - base);
   const int last = (int)(min(min(base + block, end), start + p.tokens - t0) - base);
   const AppendRows& r = p.part[1 + which];
-  const int64_t token = t0 + base - start;   // row 0's
-  const void* const x0 = (const typename XT::storage*)r.x + token * r.xs[0] + h * r.xs[1];
-  uint8_t* const o0 = (uint8_t*)r.out + place.page * r.os[0] + place.row * r.os[1] + h * r.os[2];
   const bool inter = p.rot.interleaved;
-  const int per = 64 / p.lanes, sub = lane / p.lanes;
-  const bool on = sub < per;
+  const bool on = sub < per && h < (int)heads && u0 < r.units;
+  const int64_t token = t0 + base - start;   // row 0's
+  const typename XT::storage* const x0 = (const typename XT::storage*)r.x + token * r.xs[0];
+  uint8_t* const o0 = (uint8_t*)r.out + place.page * r.os[0] + place.row * r.os[1];
   uint8_t* const sp = p.block_scale[which] + place.page * p.block_stride[which][0] +
                       (uint32_t)place.row / (uint32_t)block * p.block_stride[which][1] + h * p.block_stride[which][2];
-  const int old = first > 0 ? (int)sp[0] - 127 : 0;
+  const int old = on && first > 0 ? (int)sp[0] - 127 : 0;
 
-  // The pieces of one unit of a row, as they come and turned.
+  // The pieces of a unit of row `row`, and their values turned.
   auto load = [&](int row, const Unit& x, Piece<W>& a, Piece<W>& z) {
-    a = load_piece<XT, W>(x0, row * r.xs[0] + x.lo * r.xs[2]);
-    z = x.hi >= 0 ? load_piece<XT, W>(x0, row * r.xs[0] + x.hi * r.xs[2]) : Piece<W>{};
+    const typename XT::storage* const src = x0 + row * r.xs[0];
+    a = load_piece<XT, W>(src, lane_offset<W>(h, r.xs[1], x.lo, r.xs[2]));
+    z = x.hi >= 0 ? load_piece<XT, W>(src, lane_offset<W>(h, r.xs[1], x.hi, r.xs[2])) : Piece<W>{};
   };
-  auto turned = [&](int row, int u, const Unit& x, const Piece<W>& a, const Piece<W>& z, float (&f)[W], float (&g)[W]) {
+  auto turned = [&](int row, int u, const Unit& x, Piece<W> a, Piece<W> z, float (&f)[W], float (&g)[W]) {
     widen<XT, W>(a, f);
     widen<XT, W>(z, g);
-    if (x.turns) {
-      float c[W], s[W];
-      load_trig<W>(p, token + row, base + row, u * W, c, s);
-      turn<W>(f, g, c, s, inter);
-    }
+    if (!x.turns) return;
+    float c[W], s[W];
+    load_trig<TT, POS, W>(p, token + row, base + row, u * W, c, s);
+    turn<W>(f, g, c, s, inter);
   };
   auto largest = [&](float most, const float (&f)[W], const float (&g)[W]) {
 #pragma unroll
@@ -473,119 +507,98 @@ FA_DEV void own_block(const AppendParams& p, uint32_t w, int lane) {
     }
     return most;
   };
-  // The block's scale from its rows' largest magnitude; rows of the request
-  // before the new ones are coded again where it grows.
-  auto settle = [&](float most) {
-    const int e = block_exponent(wave_max(most));
-    if (first == 0) return e;
-    if (old >= e) return old;
-    if (on) {
-      for (int row = sub; row < first; row += per) {
-        for (int u = lane % p.lanes; u < r.units; u += p.lanes) {
-          const Unit x = unit_of<W>(r, inter, u);
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int place = i ? x.hi : x.lo;
-            if (place < 0) continue;
-            uint8_t* const at = o0 + row * r.os[1] + place * r.os[3];
-            float f[W];
-            load_codes<W>(at, f);
-#pragma unroll
-            for (int j = 0; j < W; ++j) f[j] = ldexpf(f[j], old - e);
-            store_codes<W>(at, f);
-          }
-        }
-      }
-    }
-    return e;
-  };
+  auto code_at = [&](int row, int e) { return o0 + row * r.os[1] + lane_offset<W>(h, r.os[2], e, r.os[3]); };
   auto store = [&](int row, const Unit& x, float (&f)[W], float (&g)[W], float inverse) {
 #pragma unroll
     for (int j = 0; j < W; ++j) f[j] *= inverse, g[j] *= inverse;   // exact where E4M3 tells it from zero
-    uint8_t* const at = o0 + row * r.os[1];
-    store_codes<W>(at + x.lo * r.os[3], f);
-    if (x.hi >= 0) store_codes<W>(at + x.hi * r.os[3], g);
+    store_codes<W>(code_at(row, x.lo), f);
+    if (x.hi >= 0) store_codes<W>(code_at(row, x.hi), g);
   };
-  int e;
-  const int count = last - first;
-  if (W > 1 && count <= per) {
-    // One row a lane (a decode step's one): the turned values stay.
-    const int u = lane % p.lanes, row = first + sub;
-    const bool mine = on && u < r.units && sub < count;
-    const Unit x = unit_of<W>(r, inter, u);
-    float f[W], g[W], most = 0.0f;
-    if (mine) {
-      Piece<W> a, z;
-      load(row, x, a, z);
-      turned(row, u, x, a, z, f, g);
-      most = largest(most, f, g);
-    }
-    e = settle(most);
-    if (mine) store(row, x, f, g, ldexpf(1.0f, -e));
-  } else if (W > 1 && count <= HOLD * per) {
-    const int u = lane % p.lanes;
-    const bool mine = on && u < r.units;
-    const Unit x = unit_of<W>(r, inter, u);
-    Piece<W> a[HOLD], z[HOLD];
+  // This wave's rows: first + wave, and every `waves` on.
+  const bool held = W > 1 && block <= HOLD * waves;
+  Piece<W> a[HOLD], z[HOLD];
+  float f[W], g[W], most = 0.0f;
+  const Unit x = unit_of<W>(r, inter, u0);
+  if (held) {
 #pragma unroll
     for (int i = 0; i < HOLD; ++i)
-      if (mine && i * per + sub < count) load(first + i * per + sub, x, a[i], z[i]);
-    float most = 0.0f;
+      if (on && first + wave + i * waves < last) load(first + wave + i * waves, x, a[i], z[i]);
 #pragma unroll
     for (int i = 0; i < HOLD; ++i) {
-      if (!(mine && i * per + sub < count)) continue;
-      float f[W], g[W];
-      turned(first + i * per + sub, u, x, a[i], z[i], f, g);
+      const int row = first + wave + i * waves;
+      if (!on || row >= last) continue;
+      turned(row, u0, x, a[i], z[i], f, g);
       most = largest(most, f, g);
     }
-    e = settle(most);
-    const float inverse = ldexpf(1.0f, -e);
+  } else if (on) {
+    for (int row = first + wave; row < last; row += waves)
+      for (int u = u0; u < r.units; u += p.lanes) {
+        const Unit y = unit_of<W>(r, inter, u);
+        load(row, y, a[0], z[0]);
+        turned(row, u, y, a[0], z[0], f, g);
+        most = largest(most, f, g);
+      }
+  }
+  // A head's largest magnitude, from its lanes in all the waves (the bits of
+  // positive floats are in their order).
+  if ((int)threadIdx.x < per) most_of[threadIdx.x] = 0;
+  __syncthreads();
+  if (on) atomicMax(&most_of[sub], __float_as_uint(most));
+  __syncthreads();
+  if (!on) return;
+  // The block's scale; rows of the request before the new ones are coded again
+  // where it grows.
+  int e = block_exponent(__uint_as_float(most_of[sub]));
+  if (first > 0 && old >= e) {
+    e = old;
+  } else if (first > 0) {
+    for (int row = wave; row < first; row += waves)
+      for (int u = u0; u < r.units; u += p.lanes) {
+        const Unit y = unit_of<W>(r, inter, u);
+        for (int at = y.lo;; at = y.hi) {
+          float v[W];
+          load_codes<W>(code_at(row, at), v);
 #pragma unroll
-    for (int i = 0; i < HOLD; ++i) {
-      if (!(mine && i * per + sub < count)) continue;
-      float f[W], g[W];
-      turned(first + i * per + sub, u, x, a[i], z[i], f, g);
-      store(first + i * per + sub, x, f, g, inverse);
-    }
-  } else {
-    // Long blocks and pieces of one element: the rows are read twice.
-    auto each = [&](auto use) {
-      if (!on) return;
-      for (int row = first + sub; row < last; row += per) {
-        for (int u = lane % p.lanes; u < r.units; u += p.lanes) {
-          const Unit x = unit_of<W>(r, inter, u);
-          Piece<W> a, z;
-          load(row, x, a, z);
-          float f[W], g[W];
-          turned(row, u, x, a, z, f, g);
-          use(row, x, f, g);
+          for (int j = 0; j < W; ++j) v[j] = ldexpf(v[j], old - e);
+          store_codes<W>(code_at(row, at), v);
+          if (at == y.hi || y.hi < 0) break;
         }
       }
-    };
-    float most = 0.0f;
-    each([&](int, const Unit&, float (&f)[W], float (&g)[W]) { most = largest(most, f, g); });
-    e = settle(most);
-    const float inverse = ldexpf(1.0f, -e);
-    each([&](int row, const Unit& x, float (&f)[W], float (&g)[W]) { store(row, x, f, g, inverse); });
   }
-  if (lane == 0) sp[0] = (uint8_t)(e + 127);
+  const float inverse = ldexpf(1.0f, -e);
+  if (held) {
+#pragma unroll
+    for (int i = 0; i < HOLD; ++i) {
+      const int row = first + wave + i * waves;
+      if (row >= last) continue;
+      turned(row, u0, x, a[i], z[i], f, g);
+      store(row, x, f, g, inverse);
+    }
+  } else {
+    for (int row = first + wave; row < last; row += waves)
+      for (int u = u0; u < r.units; u += p.lanes) {
+        const Unit y = unit_of<W>(r, inter, u);
+        load(row, y, a[0], z[0]);
+        turned(row, u, y, a[0], z[0], f, g);
+        store(row, y, f, g, inverse);
+      }
+  }
+  if (wave == 0 && u0 == 0) sp[0] = (uint8_t)(e + 127);
 }
 
-template <typename XT, int CACHE, int W>
-__global__ __launch_bounds__(THREADS) void append_kernel(const AppendParams p) {
+template <typename XT, typename TT, int CACHE, bool POS, int W>
+__global__ __launch_bounds__(CACHE == CACHE_BLOCK ? MOST_THREADS : THREADS) void append_kernel(const AppendParams p) {
   const int lane = threadIdx.x & 63;
-  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   uint32_t group = blockIdx.x;
   if constexpr (CACHE == CACHE_BLOCK) {
-    const uint32_t groups = (p.block_waves + WAVES - 1) / WAVES;
-    if (group < groups) {
-      const uint32_t w = group * WAVES + wave;
-      if (w < p.block_waves) own_block<XT, W>(p, w, lane);
+    __shared__ uint32_t most[64];
+    if (group < p.block_groups) {
+      own_block<XT, TT, POS, W>(p, group, lane, most);
       return;
     }
-    group -= groups;
+    group -= p.block_groups;
   }
-  token_rows<XT, CACHE, W>(p, group * WAVES + wave, lane);
+  token_rows<XT, TT, CACHE, POS, W>(p, group * (blockDim.x >> 6) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane);
 }
 
 // ------------------------------------------------------------ host
@@ -641,7 +654,9 @@ bool pieces_aligned(const AppendRows& p, int esz, int osz) {
     if ((p.xs[i] * esz) % 16) return false;
   for (int i = 0; i < 3; ++i)
     if (p.os[i] % w) return false;
-  return true;
+  // Offsets within a row stay below 2^29 elements.
+  const int64_t most = (int64_t)1 << 29;
+  return p.heads * p.xs[1] + p.dim < most && p.heads * p.os[2] + p.dim < most && p.xs[1] >= 0 && p.os[2] >= 0;
 }
 
 // Whether cos and sin come in aligned pieces wherever a unit's start in their rows.
@@ -651,21 +666,37 @@ bool trig_aligned(const fa_rotation& r) {
          (uintptr_t)r.sin_table % 16 == 0 && (r.cos_stride[0] * esz) % 16 == 0 && (r.sin_stride[0] * esz) % 16 == 0;
 }
 
-template <typename XT, int W>
+template <typename XT, typename TT, bool POS, int W>
 void launch_append(int cache, const AppendParams& p, uint32_t groups, hipStream_t s) {
-  const dim3 grid(groups), block(THREADS);
+  const dim3 grid(groups), block(p.threads);
   switch (cache) {
-    case CACHE_NONE: hipLaunchKernelGGL((append_kernel<XT, CACHE_NONE, W>), grid, block, 0, s, p); break;
-    case CACHE_SAME: hipLaunchKernelGGL((append_kernel<XT, CACHE_SAME, W>), grid, block, 0, s, p); break;
-    case CACHE_E4M3: hipLaunchKernelGGL((append_kernel<XT, CACHE_E4M3, W>), grid, block, 0, s, p); break;
-    default: hipLaunchKernelGGL((append_kernel<XT, CACHE_BLOCK, W>), grid, block, 0, s, p); break;
+    case CACHE_NONE:   // (always by positions)
+      if constexpr (POS) hipLaunchKernelGGL((append_kernel<XT, TT, CACHE_NONE, POS, W>), grid, block, 0, s, p);
+      break;
+    case CACHE_SAME: hipLaunchKernelGGL((append_kernel<XT, TT, CACHE_SAME, POS, W>), grid, block, 0, s, p); break;
+    case CACHE_E4M3: hipLaunchKernelGGL((append_kernel<XT, TT, CACHE_E4M3, POS, W>), grid, block, 0, s, p); break;
+    default: hipLaunchKernelGGL((append_kernel<XT, TT, CACHE_BLOCK, POS, W>), grid, block, 0, s, p); break;
   }
+}
+
+// Vectors with fp32 tables or tables of the rows' type; single elements else.
+template <typename XT, bool POS>
+void launch_typed(int cache, bool vec, const AppendParams& p, uint32_t groups, hipStream_t s) {
+  if (!vec) launch_append<XT, F32T, POS, 1>(cache, p, groups, s);
+  else if (XT::id == FA_F32 || (p.rot.cos_table && p.rot.trig_dtype == XT::id)) launch_append<XT, XT, POS, 16 / XT::bytes>(cache, p, groups, s);
+  else launch_append<XT, F32T, POS, 16 / XT::bytes>(cache, p, groups, s);
+}
+
+template <typename XT>
+void launch_rows(int cache, bool vec, const AppendParams& p, uint32_t groups, hipStream_t s) {
+  if (p.rot.positions) launch_typed<XT, true>(cache, vec, p, groups, s);
+  else launch_typed<XT, false>(cache, vec, p, groups, s);
 }
 
 // Fills in what the parts have in common and launches.
 int run_append(AppendParams& p, int dtype, int cache, void* stream, const char* who) {
   const int esz = dtype == FA_F32 ? 4 : 2;
-  bool vec = !p.rot.cos_table || trig_aligned(p.rot);
+  bool vec = !p.rot.cos_table || (trig_aligned(p.rot) && (p.rot.trig_dtype == FA_F32 || p.rot.trig_dtype == dtype));
   for (int i = 0; i < 3; ++i) {
     AppendRows& r = p.part[i];
     const bool cached = cache != CACHE_NONE && i > 0;
@@ -680,30 +711,37 @@ int run_append(AppendParams& p, int dtype, int cache, void* stream, const char* 
     units = r.units > units ? r.units : units;
   }
   p.lanes = units < 64 ? units : 64;
+  p.per = 64 / p.lanes;
+  p.lane_part = (65536u + (uint32_t)p.lanes - 1) / (uint32_t)p.lanes;
   int64_t passes = 0;
   for (int i = 0; i < 3; ++i) {
-    p.passes[i] = cache == CACHE_BLOCK && i > 0 ? 0 : (int)fa_ceil_div(p.part[i].heads, 64 / p.lanes);
+    p.passes[i] = cache == CACHE_BLOCK && i > 0 ? 0 : (int)fa_ceil_div(p.part[i].heads, p.per);
     passes += p.passes[i];
   }
   // A few tokens: every pass over a token's rows on a wave of its own, for the
-  // shortest chain.  Many: BATCH passes a wave, which finds its request, position
-  // and cos/sin once for them.
-  p.token_waves = (uint32_t)(passes == 0 ? 1 : p.tokens * passes <= 4096 ? passes : fa_ceil_div(passes, BATCH));
-  int64_t groups = passes ? fa_ceil_div(p.tokens * p.token_waves, WAVES) : 0;
+  // shortest chain.  Many: a wave a token, which finds its request, position and
+  // cos/sin once.
+  p.token_waves = (uint32_t)(passes > 0 && p.tokens * passes <= 4096 ? passes : 1);
   FA_REQUIRE(p.tokens * p.token_waves <= INT32_MAX, "%s: too many rows", who);
+  p.threads = THREADS;
+  int64_t groups = 0;
   if (cache == CACHE_BLOCK) {
-    const int64_t waves = (p.tokens / p.block + 2 * (int64_t)p.batch) * 2 * p.part[1].heads;
-    FA_REQUIRE(waves <= INT32_MAX, "%s: too many blocks", who);
-    p.block_waves = (uint32_t)waves;
-    groups += fa_ceil_div(waves, WAVES);
+    // As many waves as hold a block's rows in HOLD rounds, so that they are read
+    // once (blocks past that, and single elements: twice).
+    while (p.threads < MOST_THREADS && p.block > HOLD * (int)(p.threads / 64)) p.threads *= 2;
+    p.head_sets = (int32_t)fa_ceil_div(p.part[1].heads, p.per);
+    groups = (p.tokens / p.block + 2 * (int64_t)p.batch) * 2 * p.head_sets;
+    FA_REQUIRE(groups <= INT32_MAX, "%s: too many blocks", who);
+    p.block_groups = (uint32_t)groups;
   }
-  FA_REQUIRE(groups < 1ll << 24, "%s: too many rows", who);   // 2^32 threads a launch
+  if (passes) groups += fa_ceil_div(p.tokens * p.token_waves, p.threads / 64);
+  FA_REQUIRE(groups * p.threads < 1ll << 32, "%s: too many rows", who);   // 2^32 threads a launch
   if (groups == 0) return FA_OK;
   hipStream_t s = (hipStream_t)stream;
   switch (dtype) {
-    case FA_F16: vec ? launch_append<F16T, 8>(cache, p, groups, s) : launch_append<F16T, 1>(cache, p, groups, s); break;
-    case FA_BF16: vec ? launch_append<BF16T, 8>(cache, p, groups, s) : launch_append<BF16T, 1>(cache, p, groups, s); break;
-    default: vec ? launch_append<F32T, 4>(cache, p, groups, s) : launch_append<F32T, 1>(cache, p, groups, s); break;
+    case FA_F16: launch_rows<F16T>(cache, vec, p, (uint32_t)groups, s); break;
+    case FA_BF16: launch_rows<BF16T>(cache, vec, p, (uint32_t)groups, s); break;
+    default: launch_rows<F32T>(cache, vec, p, (uint32_t)groups, s); break;
   }
   return fa_check_launch(who);
 }
