@@ -85,16 +85,14 @@ struct Place {
   int row;
 };
 
+// (Without a branch past the first: the table's load need not be waited for
+// where the place is not yet used.)
 FA_DEV Place place_of(const AppendParams& p, int b, int64_t pos) {
-  Place x{-1, 0};
-  if (pos < 0 || pos > INT32_MAX) return x;
-  const uint32_t column = (uint32_t)pos / (uint32_t)p.page_size;
-  if ((int64_t)column >= p.table_cols) return x;
-  const int64_t page = load_invariant_i32(p.table, b * p.bt_stride[0] + (int64_t)column * p.bt_stride[1]);
-  if (page < 0 || page >= p.num_pages) return x;
-  x.page = page;
-  x.row = (int)((uint32_t)pos - column * (uint32_t)p.page_size);
-  return x;
+  if (p.table_cols == 0) return Place{-1, 0};
+  const uint32_t size = (uint32_t)p.page_size, at = pos < 0 || pos > INT32_MAX ? 0u : (uint32_t)pos, column = at / size;
+  const bool in = at == pos && (int64_t)column < p.table_cols;
+  const int64_t page = load_invariant_i32(p.table, b * p.bt_stride[0] + (in ? (int64_t)column : 0) * p.bt_stride[1]);
+  return Place{in && page >= 0 && page < p.num_pages ? page : -1, (int)(at - column * size)};
 }
 
 FA_DEV uint32_t pair_axes(const AppendParams& p, int i) {
@@ -298,19 +296,19 @@ FA_DEV void store_codes(uint8_t* out, const float (&f)[W]) {
     out[0] = f32_to_e4m3(f[0]);
   } else {
     uint32_t w[W / 4];
-    bool nan = false;
+    float probe = 0.0f;   // 0 unless a value is NaN or infinite
 #pragma unroll
     for (int j = 0; j < W; j += 4) {
       float x[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         x[k] = __builtin_amdgcn_fmed3f(f[j + k], -448.0f, 448.0f);
-        nan |= f[j + k] != f[j + k];
+        probe = fmaf(f[j + k], 0.0f, probe);
       }
       const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
       w[j / 4] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], lo, true);
     }
-    if (__builtin_expect(nan, 0)) {
+    if (__builtin_expect(probe != 0.0f, 0)) {
 #pragma unroll
       for (int j = 0; j < W; ++j)
         if (f[j] != f[j]) w[j / 4] = (w[j / 4] & ~(0xffu << (8 * (j % 4)))) | (e4m3_code(f[j]) & 0xffu) << (8 * (j % 4));
@@ -346,13 +344,7 @@ FA_DEV auto lane_offset(int h, int64_t head_stride, int e, int64_t stride) {
 
 // Passes of a wave over a token's rows whose loads are all issued before the
 // first of them is used.
-#ifndef PA_BATCH
-#define PA_BATCH 2
-#endif
-#ifndef PA_MIN
-#define PA_MIN 1
-#endif
-constexpr int BATCH = PA_BATCH;
+constexpr int BATCH = 2;
 
 template <typename XT, typename TT, int CACHE, bool POS, int W>
 FA_DEV void token_rows(const AppendParams& p, uint32_t w, int lane) {
@@ -366,15 +358,15 @@ FA_DEV void token_rows(const AppendParams& p, uint32_t w, int lane) {
   int b = -1;
   int64_t pos = -1;
   Place at{-1, 0};
-  if (CACHE != CACHE_NONE && (keeps || !POS)) {
+  bool located = CACHE == CACHE_NONE || (!keeps && POS);   // (nothing here depends on the request)
+  auto locate = [&]() {
+    located = true;
     b = last_at_most(p.batch + 1, t, lane, [&](int i) { return (int64_t)cu_at(p, i); });
     if (b >= p.batch) b = -1;
-    if (b >= 0) {
-      pos = (int64_t)load_invariant_i32(p.used, b * p.used_stride) - cu_of(p, b + 1) + t;
-      if (keeps) at = place_of(p, b, pos);
-    }
-  }
-  const bool q_turns = CACHE == CACHE_NONE || POS || b >= 0;
+    if (b < 0) return;
+    pos = (int64_t)load_invariant_i32(p.used, b * p.used_stride) - cu_of(p, b + 1) + t;
+    if (keeps) at = place_of(p, b, pos);
+  };
   for (int u = u0; u < 256; u += 64) {   // (one round but for pieces of one element)
     float c[W], s[W];
     bool have = false;
@@ -387,13 +379,14 @@ FA_DEV void token_rows(const AppendParams& p, uint32_t w, int lane) {
         const int which = pass < p.passes[0] ? 0 : pass < p.passes[0] + p.passes[1] ? 1 : 2;
         const int h = (pass - (which > 0 ? p.passes[0] : 0) - (which > 1 ? p.passes[1] : 0)) * per + sub;
         const AppendRows& r = p.part[which];
-        on[k] = pass < total && sub < per && h < r.heads && u < r.units && (CACHE == CACHE_NONE || which == 0 || at.page >= 0);
+        on[k] = pass < total && sub < per && h < r.heads && u < r.units;
         if (!on[k]) continue;
         const Unit x = unit_of<W>(r, inter, u);
         const void* const src = (const typename XT::storage*)r.x + t * r.xs[0];
         a[k] = load_piece<XT, W>(src, lane_offset<W>(h, r.xs[1], x.lo, r.xs[2]));
         z[k] = x.hi >= 0 ? load_piece<XT, W>(src, lane_offset<W>(h, r.xs[1], x.hi, r.xs[2])) : a[k];
       }
+      if (!located) locate();   // behind the first rows' loads, which need not wait for it
       // (Parts that do not turn come last, so a batch that turns starts with one that does.)
       if (!have && u * W < p.part[s0 < p.passes[0] ? 0 : 1].half && s0 < p.passes[0] + p.passes[1]) {
         load_trig<TT, POS, W>(p, t, pos, u * W, c, s);
@@ -408,7 +401,8 @@ FA_DEV void token_rows(const AppendParams& p, uint32_t w, int lane) {
         const AppendRows& r = p.part[which];
         const Unit x = unit_of<W>(r, inter, u);
         const bool cached = CACHE != CACHE_NONE && which > 0;
-        const bool turns = x.turns && (cached || q_turns);
+        if (cached && at.page < 0) continue;
+        const bool turns = x.turns && (cached || CACHE == CACHE_NONE || POS || b >= 0);
         const int64_t dst = cached ? at.page * r.os[0] + at.row * r.os[1] : t * r.os[1];
         const auto lo = lane_offset<W>(h, r.os[2], x.lo, r.os[3]), hi = lane_offset<W>(h, r.os[2], x.hi, r.os[3]);
         const bool codes = CACHE == CACHE_E4M3 && cached;
@@ -469,8 +463,7 @@ FA_DEV void own_block(const AppendParams& p, uint32_t group, int lane, uint32_t*
   if (t0 < 0 || n <= 0 || end <= 0) return;
   const int64_t base = ((uint32_t)from / (uint32_t)block + (int64_t)(id - t0 / block - 2 * b)) * block;   // its first position
   if (base >= end || base - start >= p.tokens - t0) return;
-  const Place place = place_of(p, b, base);
-  if (place.page < 0) return;   // (so far the same for the whole workgroup)
+  const Place place = place_of(p, b, base);   // (used behind the rows' loads)
   // The block's new rows (none past the last row there is).
   const int first = (int)(max(base, from) - base);
   const int last = (int)(min(min(base + block, end), start + p.tokens - t0) - base);
@@ -479,11 +472,6 @@ FA_DEV void own_block(const AppendParams& p, uint32_t group, int lane, uint32_t*
   const bool on = sub < per && h < (int)heads && u0 < r.units;
   const int64_t token = t0 + base - start;   // row 0's
   const typename XT::storage* const x0 = (const typename XT::storage*)r.x + token * r.xs[0];
-  uint8_t* const o0 = (uint8_t*)r.out + place.page * r.os[0] + place.row * r.os[1];
-  uint8_t* const sp = p.block_scale[which] + place.page * p.block_stride[which][0] +
-                      (uint32_t)place.row / (uint32_t)block * p.block_stride[which][1] + h * p.block_stride[which][2];
-  const int old = on && first > 0 ? (int)sp[0] - 127 : 0;
-
   // The pieces of a unit of row `row`, and their values turned.
   auto load = [&](int row, const Unit& x, Piece<W>& a, Piece<W>& z) {
     const typename XT::storage* const src = x0 + row * r.xs[0];
@@ -498,21 +486,20 @@ FA_DEV void own_block(const AppendParams& p, uint32_t group, int lane, uint32_t*
     load_trig<TT, POS, W>(p, token + row, base + row, u * W, c, s);
     turn<W>(f, g, c, s, inter);
   };
+  // The largest finite magnitude (a maximum leaves NaN out; infinities are rare).
   auto largest = [&](float most, const float (&f)[W], const float (&g)[W]) {
+    float all = 0.0f;
 #pragma unroll
-    for (int j = 0; j < W; ++j) {
-      const float a = fabsf(f[j]), z = fabsf(g[j]);
-      most = fmaxf(most, a < INFINITY ? a : 0.0f);
-      most = fmaxf(most, z < INFINITY ? z : 0.0f);
+    for (int j = 0; j < W; ++j) all = fmaxf(all, fmaxf(fabsf(f[j]), fabsf(g[j])));
+    if (__builtin_expect(all == INFINITY, 0)) {
+      all = 0.0f;
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        const float a = fabsf(f[j]), z = fabsf(g[j]);
+        all = fmaxf(all, fmaxf(a < INFINITY ? a : 0.0f, z < INFINITY ? z : 0.0f));
+      }
     }
-    return most;
-  };
-  auto code_at = [&](int row, int e) { return o0 + row * r.os[1] + lane_offset<W>(h, r.os[2], e, r.os[3]); };
-  auto store = [&](int row, const Unit& x, float (&f)[W], float (&g)[W], float inverse) {
-#pragma unroll
-    for (int j = 0; j < W; ++j) f[j] *= inverse, g[j] *= inverse;   // exact where E4M3 tells it from zero
-    store_codes<W>(code_at(row, x.lo), f);
-    if (x.hi >= 0) store_codes<W>(code_at(row, x.hi), g);
+    return fmaxf(most, all);
   };
   // This wave's rows: first + wave, and every `waves` on.
   const bool held = W > 1 && block <= HOLD * waves;
@@ -539,6 +526,18 @@ FA_DEV void own_block(const AppendParams& p, uint32_t group, int lane, uint32_t*
         most = largest(most, f, g);
       }
   }
+  if (place.page < 0) return;   // (like the returns before it, the same for the whole workgroup)
+  uint8_t* const o0 = (uint8_t*)r.out + place.page * r.os[0] + place.row * r.os[1];
+  uint8_t* const sp = p.block_scale[which] + place.page * p.block_stride[which][0] +
+                      (uint32_t)place.row / (uint32_t)block * p.block_stride[which][1] + h * p.block_stride[which][2];
+  const int old = on && first > 0 ? (int)sp[0] - 127 : 0;
+  auto code_at = [&](int row, int e) { return o0 + row * r.os[1] + lane_offset<W>(h, r.os[2], e, r.os[3]); };
+  auto store = [&](int row, const Unit& x, float (&f)[W], float (&g)[W], float inverse) {
+#pragma unroll
+    for (int j = 0; j < W; ++j) f[j] *= inverse, g[j] *= inverse;   // exact where E4M3 tells it from zero
+    store_codes<W>(code_at(row, x.lo), f);
+    if (x.hi >= 0) store_codes<W>(code_at(row, x.hi), g);
+  };
   // A head's largest magnitude, from its lanes in all the waves (the bits of
   // positive floats are in their order).
   if ((int)threadIdx.x < per) most_of[threadIdx.x] = 0;
