@@ -28,7 +28,6 @@ kernel variant depends only on dtypes, head dims and feature flags, and a
 key tile that a row cannot see adds exact zeros to its sums.  So a request's
 rows are bit-identical whatever else is in the batch.
 """
-import ctypes
 import math
 
 import torch
@@ -120,9 +119,7 @@ def _entry(p, name, a):
     cache has its own (fa_block_*), with the scales beside the attention's."""
     if not p.block_scaled:
         return name, a
-    k, v = p.k_descale, p.v_descale
-    block = _lib.BlockAttnArgs(ctypes.sizeof(_lib.BlockAttnArgs), a, k.data_ptr(), v.data_ptr(), k.stride(), v.stride(),
-                               p.k.shape[1] // k.shape[1])
+    block = _lib.block_attn(a, p.k_descale, p.v_descale, p.k.shape[1] // p.k_descale.shape[1])
     return name.replace("fa_", "fa_block_", 1), block
 
 

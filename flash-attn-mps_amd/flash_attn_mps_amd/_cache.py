@@ -22,7 +22,7 @@ from functools import lru_cache
 import torch
 
 from . import _lib
-from ._problem import Want, on_gpu, reject_training
+from ._problem import _check, on_gpu, reject_training
 
 _INPUT_TYPES = (torch.float16, torch.bfloat16, torch.float32)
 BLOCK_SCALE = torch.float8_e8m0fnu
@@ -102,7 +102,7 @@ def _write_desc(x, cache, scale, x_strides, keep):
 
 def _check_cache_shape(x, cache, row_dims):
     """cache [pages, page_size, heads, dim] matching the (heads, dim) of x."""
-    if cache.ndim != 4 or tuple(cache.shape[2:]) != tuple(x.shape[row_dims:]):
+    if cache.ndim != 4 or cache.shape[2:] != x.shape[row_dims:]:
         raise ValueError(f"cache {tuple(cache.shape)} must be [pages, page_size, {x.shape[-2]}, {x.shape[-1]}]")
 
 
@@ -384,34 +384,37 @@ def append_paged_kvcache(k, v, k_cache, v_cache, cu_seqlens_q, seqused_k, block_
     """The rows of each request, its last seqused_k[b] positions, into its pages (see the package's function)."""
     reject_training(tensors=(k, v, k_cache, v_cache, q, cos, sin))
     _check_rows(k=k, v=v, q=q)
-    tokens, heads = k.shape[:2]
-    device = k.device
+    tokens, heads, dim_k = k.shape
+    device, dtype, shape = k.device, k.dtype, k_cache.shape
+    fp8 = k_cache.dtype == torch.float8_e4m3fn
     if v.shape[1] != heads:
         raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must have the same heads")
     for name, x, cache in (("k_cache", k, k_cache), ("v_cache", v, v_cache)):
         if cache.device != device:
             raise ValueError(f"{name} is on {cache.device}; expected {device}")
         _check_cache_shape(x, cache, 1)
-        if cache.dtype != k.dtype and cache.dtype != torch.float8_e4m3fn:
-            raise TypeError(f"a {cache.dtype} cache cannot take {k.dtype} rows (use the same dtype or float8_e4m3fn)")
-    pages, size = k_cache.shape[:2]
-    if v_cache.shape[:2] != k_cache.shape[:2] or v_cache.dtype != k_cache.dtype or size < 1:
+        if cache.dtype != dtype and cache.dtype != torch.float8_e4m3fn:
+            raise TypeError(f"a {cache.dtype} cache cannot take {dtype} rows (use the same dtype or float8_e4m3fn)")
+    pages, size = shape[0], shape[1]
+    if v_cache.shape[:2] != shape[:2] or v_cache.dtype != k_cache.dtype or size < 1:
         raise ValueError("the K and V caches must have the same pages, page size and type")
-    batch = seqused_k.shape[0] if torch.is_tensor(seqused_k) and seqused_k.ndim == 1 else -1
-    for t, name, shape in ((cu_seqlens_q, "cu_seqlens_q", (batch + 1,)), (seqused_k, "seqused_k", (batch,)),
-                           (block_table, "block_table", (batch, None))):
-        if not torch.is_tensor(t) or batch < 0:
+    for t in (cu_seqlens_q, seqused_k, block_table):
+        if not torch.is_tensor(t):
             raise ValueError("cu_seqlens_q, seqused_k and block_table are int32 tensors [B + 1], [B] and [B, pages]")
-        Want(name, shape, (torch.int32,)).check(t, device)
-    if is_block_scale(k_scale) != is_block_scale(v_scale):
+    batch = seqused_k.numel()
+    _check(seqused_k, "seqused_k", (batch,), (torch.int32,), device)
+    _check(cu_seqlens_q, "cu_seqlens_q", (batch + 1,), (torch.int32,), device)
+    _check(block_table, "block_table", (batch, None), (torch.int32,), device)
+    blocks = is_block_scale(k_scale)
+    if blocks != is_block_scale(v_scale):
         raise ValueError("k_scale and v_scale are both scales per block (float8_e8m0fnu) or neither")
-    keep, block, block_ptrs, block_strides, head_scale = [], 0, (0, 0), (0,) * 6, ((0, 0), (0, 0))
-    if is_block_scale(k_scale):
+    block, block_ptrs, block_strides, head_scale = 0, (0, 0), (0,) * 6, ((0, 0), (0, 0))
+    if blocks:
         block = block_of(k_cache, k_scale, "k_scale")
         if block_of(v_cache, v_scale, "v_scale") != block:
             raise ValueError("the K and V scales must have the same tokens per block")
         block_ptrs, block_strides = (k_scale.data_ptr(), v_scale.data_ptr()), (*k_scale.stride(), *v_scale.stride())
-    elif k_cache.dtype == torch.float8_e4m3fn:
+    elif fp8:
         keep = [_per_head_scale(s, heads, device) for s in (k_scale, v_scale)]
         head_scale = [(s.data_ptr(), stride) for s, stride in keep]
     if (cos is None) != (sin is None):
@@ -425,14 +428,13 @@ def append_paged_kvcache(k, v, k_cache, v_cache, cu_seqlens_q, seqused_k, block_
                         [k.shape[2]] if q is None else [k.shape[2], q.shape[2]], device)
     out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=device)
     if tokens:
-        code = _lib.DTYPE_CODE
-        descs = []
-        for x, cache, (scale, stride) in ((k, k_cache, head_scale[0]), (v, v_cache, head_scale[1])):
-            descs += (x.data_ptr(), cache.data_ptr(), scale, code[x.dtype], code[cache.dtype], heads, x.shape[2],
-                      *x.stride(), *cache.stride(), stride)
-        a = _lib.pack_append(*descs, *block_ptrs, *block_strides, block, *(_NO_ROWS if q is None else _rows(q, out)), *rot,
-                             cu_seqlens_q.data_ptr(), cu_seqlens_q.stride(0), seqused_k.data_ptr(), seqused_k.stride(0),
-                             block_table.data_ptr(), *block_table.stride(), tokens, batch, size, pages,
-                             block_table.shape[1])
+        x_code, c_code = _lib.DTYPE_CODE[dtype], _lib.DTYPE_CODE[k_cache.dtype]
+        (k_s, k_st), (v_s, v_st) = head_scale
+        a = _lib.pack_append(
+            k.data_ptr(), k_cache.data_ptr(), k_s, x_code, c_code, heads, dim_k, *k.stride(), *k_cache.stride(), k_st,
+            v.data_ptr(), v_cache.data_ptr(), v_s, x_code, c_code, heads, v.shape[2], *v.stride(), *v_cache.stride(), v_st,
+            *block_ptrs, *block_strides, block, *(_NO_ROWS if q is None else _rows(q, out)), *rot,
+            cu_seqlens_q.data_ptr(), *cu_seqlens_q.stride(), seqused_k.data_ptr(), *seqused_k.stride(),
+            block_table.data_ptr(), *block_table.stride(), tokens, batch, size, pages, block_table.shape[1])
         _lib.call("fa_paged_append", a, device)
     return out

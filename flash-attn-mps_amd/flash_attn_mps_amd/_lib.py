@@ -177,6 +177,17 @@ class MergePartialsArgs(ctypes.Structure):
 _rotary_packer, _append_packer = _packer(RotaryRowsArgs), _packer(PagedAppendArgs)
 
 
+_block_tail = struct.Struct("@PP7q")
+_BLOCK_SIZE = struct.pack("@q", ctypes.sizeof(BlockAttnArgs))
+assert ctypes.sizeof(BlockAttnArgs) == 8 + ctypes.sizeof(AttnArgs) + _block_tail.size
+
+
+def block_attn(a, k_scale, v_scale, block):
+    """A BlockAttnArgs: AttnArgs `a` over a cache with these scales, `block` tokens each."""
+    return BlockAttnArgs.from_buffer_copy(b"".join((
+        _BLOCK_SIZE, a, _block_tail.pack(k_scale.data_ptr(), v_scale.data_ptr(), *k_scale.stride(), *v_scale.stride(), block))))
+
+
 def pack_rotary_rows(*values):
     """A RotaryRowsArgs from its fields' values after `size`."""
     return _pack(RotaryRowsArgs, _rotary_packer, "rotary", (_rotary_packer.size, *values))
