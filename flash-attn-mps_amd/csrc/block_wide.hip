@@ -1,0 +1,232 @@
+// Prefill over a block-scaled cache by way of 16-bit rows: one pass widens the
+// keys and values that the batch sees to the queries' type in a workspace, the
+// 16-bit prefill kernels run on that, and rows that met a value that is not
+// finite run again by block_row.
+//
+// A value times its power of two is exact in bf16, and in fp16 to fp16's own
+// range.  The E4M3 tiles widen every key tile again for each block of query
+// rows; with many rows a key that costs more than this pass, which HBM bounds: 3
+// bytes a value, 36K keys of 8 heads x 128, K and V, 225 MB.
+#include "block_row.h"
+
+namespace {
+
+constexpr int TILE = 64;   // keys of a workgroup
+
+struct WideParams {
+  fa_block_attn a;
+  uint16_t* out[2];       // [batch, capacity, heads, dim], K and V
+  int32_t* flags;         // [batch, tiles, 2]: whether a tile may hold values that are not finite
+  int64_t capacity;
+  int32_t tiles, bf16;
+  int32_t chunks[2];      // pieces of a head's row
+  uint32_t limit;         // scale bytes above it may leave the 16-bit type's range
+};
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
+
+// Four codes -> four 16-bit values times `scale`.
+template <bool BF16>
+FA_DEV u32x2 widen4(uint32_t w, float scale) {
+  if constexpr (BF16)
+    return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true))};
+  else
+    return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, true))};
+}
+
+// The first key of request r that some query row sees, down to a multiple of 128.
+FA_DEV int first_key(const fa_attn_args& a, const RequestInfo& r) {
+  if (a.mask_kind != 0 || a.window_left < 0) return 0;
+  return max(r.k_len - r.q_len - a.window_left, 0) & ~127;
+}
+
+FA_DEV bool runs_here(const fa_attn_args& a, const RequestInfo& r) {
+  return r.q_len > 1 || (r.q_len == 1 && !(a.flags & FA_FLAG_SKIP_SINGLE_QUERY));
+}
+
+// One workgroup per (tile, request, K or V).  A piece is CODES codes of one row
+// of one head.
+template <bool BF16, int CODES>
+__global__ __launch_bounds__(256) void widen_kernel(const WideParams p) {
+  const fa_block_attn& a = p.a;
+  const int tile = blockIdx.x, which = blockIdx.z;
+  const int64_t b = blockIdx.y;
+  const RequestInfo r = load_request(a, b);
+  const int heads = (int)a.heads_k, chunks = p.chunks[which], per_key = heads * chunks;
+  const int64_t* const st = which ? a.v_stride : a.k_stride;
+  const uint8_t* const in = (const uint8_t*)(which ? a.v : a.k);
+  const int begin = tile * TILE, end = min(begin + TILE, (int)min((int64_t)r.k_len, p.capacity));
+  bool odd = false;
+  if (runs_here(a, r) && begin >= first_key(a, r) && begin < end) {
+    const int items = (end - begin) * per_key;
+    const uint32_t size = (uint32_t)a.page_size;
+    uint16_t* const out = p.out[which] + (b * p.capacity + begin) * per_key * CODES;
+    constexpr int N = 4;   // pieces of a thread in flight
+    for (int i0 = threadIdx.x; i0 < items; i0 += N * 256) {
+      uint32_t w[N][CODES / 4], e[N];
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const int i = i0 + n * 256;
+        if (i >= items) continue;
+        const uint32_t key = (uint32_t)i / (uint32_t)per_key, rem = (uint32_t)i - key * (uint32_t)per_key;
+        const uint32_t h = rem / (uint32_t)chunks, c = rem - h * (uint32_t)chunks;
+        const uint32_t pos = (uint32_t)begin + key, column = pos / size, row = pos - column * size;
+        const int64_t page = a.block_table[b * a.bt_stride[0] + (int64_t)column * a.bt_stride[1]];
+        const uint8_t* const src = in + page * st[0] + (int64_t)row * st[1] + (int64_t)h * st[2] + c * CODES;
+        if constexpr (CODES == 16) {
+          const u32x4 v = *(const u32x4*)src;
+          w[n][0] = v[0], w[n][1] = v[1], w[n][2] = v[2], w[n][3] = v[3];
+        } else {
+          const u32x2 v = *(const u32x2*)src;
+          w[n][0] = v[0], w[n][1] = v[1];
+        }
+        e[n] = scale_byte(a, which, page, (int)row, (int)h);
+      }
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const int i = i0 + n * 256;
+        if (i >= items) continue;
+        const float scale = e8m0_to_f32(e[n]);
+        odd |= e[n] > p.limit;
+        u32x4* const dst = (u32x4*)(out + (int64_t)i * CODES);
+#pragma unroll
+        for (int k = 0; k < CODES / 4; k += 2) {
+          const u32x2 x = widen4<BF16>(w[n][k], scale), y = widen4<BF16>(w[n][k + 1], scale);
+          dst[k / 2] = u32x4{x[0], x[1], y[0], y[1]};
+          // NaN codes: 0x7f without the sign.
+          odd |= ((((w[n][k] & 0x7f7f7f7fu) + 0x01010101u) | ((w[n][k + 1] & 0x7f7f7f7fu) + 0x01010101u)) & 0x80808080u) != 0;
+        }
+      }
+    }
+  }
+  const int any = __syncthreads_or(odd);
+  if (threadIdx.x == 0) p.flags[(b * p.tiles + tile) * 2 + which] = any;
+}
+
+// Rows whose output is not finite, where some tile was flagged: a few workgroups
+// that stop after the flags in every usual call.
+template <bool BF16>
+__global__ __launch_bounds__(256) void again_kernel(const WideParams p) {
+  const fa_block_attn& a = p.a;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  bool odd = false;
+  for (int64_t i = threadIdx.x; i < a.batch * p.tiles * 2; i += 256) odd |= p.flags[i] != 0;
+  if (!__syncthreads_or(odd)) return;
+  const int Dv = (int)a.head_dim_v;
+  for (int64_t b = 0; b < a.batch; ++b) {
+    const RequestInfo r = load_request(a, b);
+    if (!runs_here(a, r)) continue;
+    for (int64_t i = (int64_t)blockIdx.x * 4 + wave; i < (int64_t)r.q_len * a.heads_q; i += (int64_t)gridDim.x * 4) {
+      const int row = (int)(i / a.heads_q), h = (int)(i - (int64_t)row * a.heads_q);
+      const int64_t tq = (int64_t)r.q_begin + row;
+      uint16_t* const out = (uint16_t*)a.out + tq * a.out_stride[0] + (int64_t)h * a.out_stride[1];
+      const uint32_t top = BF16 ? 0x7f80u : 0x7c00u;
+      bool bad = false;
+      for (int d = lane; d < Dv; d += 64) bad |= (out[d] & top) == top;
+      if (!__any(bad)) continue;
+      const float lse = block_row<4>(
+          a, b, r, h / (int)(a.heads_q / a.heads_k), h, 0, tq, row + r.k_len - r.q_len, 0, r.k_len, lane,
+          [&](int d) {
+            const uint32_t w = ((const uint16_t*)a.q)[tq * a.q_stride[0] + (int64_t)h * a.q_stride[1] + d];
+            return BF16 ? bf16_bits_to_f32(w) : f16_bits_to_f32(w);
+          },
+          [&](int d, float x) {
+            if constexpr (BF16) store_elem<BF16T>(out, d, x);
+            else store_elem<F16T>(out, d, x);
+          });
+      if (lane == 0) a.lse[(int64_t)h * a.lse_stride[0] + tq * a.lse_stride[1]] = lse != lse ? -INFINITY : lse;
+    }
+  }
+}
+
+// Codes of a piece: 16, or 8 where dims or strides ask for it; 0 where the rows
+// have no aligned pieces.
+int piece_codes(const fa_attn_args& a) {
+  for (int codes : {16, 8}) {
+    bool ok = a.head_dim_qk % codes == 0 && a.head_dim_v % codes == 0 && a.k_stride[3] == 1 && a.v_stride[3] == 1 &&
+              (uintptr_t)a.k % codes == 0 && (uintptr_t)a.v % codes == 0;
+    for (int i = 0; i < 3; ++i) ok = ok && a.k_stride[i] % codes == 0 && a.v_stride[i] % codes == 0;
+    if (ok) return codes;
+  }
+  return 0;
+}
+
+// The 16-bit call on the workspace: request b's keys are page b of pages of
+// `capacity` rows.
+fa_attn_args wide_attn(const fa_block_wide_args& w) {
+  fa_attn_args a = w.block.attn;
+  const int64_t heads = a.heads_k;
+  a.k = w.k_wide, a.v = w.v_wide;
+  a.k_dtype = a.v_dtype = a.q_dtype;
+  a.page_size = w.capacity;
+  const int64_t dims[2] = {a.head_dim_qk, a.head_dim_v};
+  for (int i = 0; i < 2; ++i) {
+    int64_t* const st = i ? a.v_stride : a.k_stride;
+    st[0] = w.capacity * heads * dims[i], st[1] = heads * dims[i], st[2] = dims[i], st[3] = 1;
+  }
+  a.block_table = w.rows;
+  a.bt_stride[0] = 1, a.bt_stride[1] = 1;
+  return a;
+}
+
+bool wide_ok(const fa_block_wide_args* w, fa_block_attn* a) {
+  if (!w || w->size != (int64_t)sizeof(fa_block_wide_args) || !fa_block_arguments(&w->block, a)) return false;
+  if ((a->q_dtype != FA_BF16 && a->q_dtype != FA_F16) || a->out_dtype != a->q_dtype) return false;
+  if (a->head_dim_v > 256 || a->batch > 65535 || a->max_seqlen_k > w->capacity || w->capacity > INT32_MAX / 2) return false;
+  if (w->capacity < 1 || !piece_codes(*a)) return false;
+  // (Rows of a wave's output are read back as they were written.)
+  if (a->out_stride[2] != 1) return false;
+  const fa_attn_args wide = wide_attn(*w);
+  return fa_prefill_supported(&wide);
+}
+
+}  // namespace
+
+extern "C" int fa_block_wide_supported(const fa_block_wide_args* args) {
+  fa_block_attn a;
+  return wide_ok(args, &a);
+}
+
+extern "C" int fa_block_wide_fwd(const fa_block_wide_args* args, void* stream) {
+  const char* who = "fa_block_wide_fwd";
+  FA_REQUIRE(args && args->size == (int64_t)sizeof(fa_block_wide_args), "%s: null or mismatched arguments", who);
+  WideParams p;
+  const int rc = fa_validate_block(&args->block, &p.a, who);
+  if (rc) return rc;
+  FA_REQUIRE(args->k_wide && args->v_wide && args->rows && args->flags, "%s: null workspace", who);
+  fa_block_attn checked;
+  if (!wide_ok(args, &checked)) {
+    fa_set_error("%s: combination not supported by the 16-bit prefill", who);
+    return FA_ERR_UNSUPPORTED;
+  }
+  if (p.a.total_q == 0) return FA_OK;
+  const bool bf16 = p.a.q_dtype == FA_BF16;
+  const int codes = piece_codes(p.a);
+  p.out[0] = (uint16_t*)args->k_wide, p.out[1] = (uint16_t*)args->v_wide;
+  p.flags = args->flags;
+  p.capacity = args->capacity;
+  p.bf16 = bf16;
+  p.tiles = (int32_t)fa_ceil_div(p.a.max_seqlen_k, TILE);
+  p.chunks[0] = (int32_t)(p.a.head_dim_qk / codes), p.chunks[1] = (int32_t)(p.a.head_dim_v / codes);
+  // 448 * 2^(e - 127) is finite in the type up to these.
+  p.limit = bf16 ? 127 + 118 : 127 + 7;
+  hipStream_t s = (hipStream_t)stream;
+  if (p.tiles > 0) {
+    const dim3 grid((unsigned)p.tiles, (unsigned)p.a.batch, 2);
+    void (*kern)(const WideParams) = codes == 16 ? (bf16 ? widen_kernel<true, 16> : widen_kernel<false, 16>)
+                                                 : (bf16 ? widen_kernel<true, 8> : widen_kernel<false, 8>);
+    hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, p);
+    const int launched = fa_check_launch(who);
+    if (launched) return launched;
+  }
+  const fa_attn_args wide = wide_attn(*args);
+  const int ran = fa_prefill_fwd(&wide, stream);
+  if (ran || p.tiles == 0) return ran;
+  hipLaunchKernelGGL((bf16 ? again_kernel<true> : again_kernel<false>), dim3(256), dim3(256), 0, s, p);
+  return fa_check_launch(who);
+}

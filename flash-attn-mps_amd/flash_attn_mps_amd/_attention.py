@@ -120,6 +120,8 @@ def _entry(p, name, a):
     if not p.block_scaled:
         return name, a
     block = _lib.block_attn(a, p.k_descale, p.v_descale, p.k.shape[1] // p.k_descale.shape[1])
+    if p.wide is not None and name.startswith("fa_prefill"):
+        return name.replace("fa_prefill", "fa_block_wide", 1), _lib.block_wide(block, *p.wide)
     return name.replace("fa_", "fa_block_", 1), block
 
 
@@ -131,6 +133,39 @@ def call(p, name, a):
 
 def supported(p, name, a):
     return _lib.supported(*_entry(p, name, a))
+
+
+# A block-scaled prefill runs by way of 16-bit rows (fa_block_wide_fwd) from this
+# many query rows and heads per KV head and request on, while the workspace stays
+# below this size.  The pass over the cache costs 3 bytes a value at 4 TB/s, the
+# E4M3 tiles about half as much again as the 16-bit ones for each row.  Measured (us, tiles
+# / by way of 16-bit rows): WIDE_FIGURES
+_WIDE_ROWS = 640
+_WIDE_BYTES = 4 << 30
+
+
+def widen(p, a):
+    """The 16-bit workspace of a block-scaled prefill as p.wide, where it pays or
+    nothing else but the generic kernel takes the call.  Calls with a fixed order
+    stay on the tiles, whose choice does not depend on the batch."""
+    if p.q.dtype not in (torch.float16, torch.bfloat16) or p.deterministic or p.max_k < 1:
+        return
+    rows, visible = p.tokens / p.batch, p.visible_max
+    shared = rows * (p.heads // p.kv_heads) * visible / min(p.max_k, visible + rows)
+    if shared < _WIDE_ROWS and supported(p, "fa_prefill_supported", a):
+        return
+    keys = p.batch * p.max_k * p.kv_heads
+    if 2 * keys * (p.dim_qk + p.dim_v) > _WIDE_BYTES:
+        return
+    from .interface import _counting
+    identity = _counting.rows(p.batch, p.device)
+    work = torch.empty(keys * (p.dim_qk + p.dim_v), dtype=p.q.dtype, device=p.device)
+    flags = torch.empty(2 * p.batch * -(-p.max_k // 64), dtype=torch.int32, device=p.device)
+    p.wide = (work.data_ptr(), work.data_ptr() + 2 * keys * p.dim_qk, p.max_k, identity.data_ptr(), flags.data_ptr())
+    if supported(p, "fa_prefill_supported", a):
+        p.keep += [identity, work, flags]
+    else:
+        p.wide = None
 
 
 def _fits_prefill(p, out):
@@ -372,8 +407,9 @@ def solve(p):
     if p.batch < 1:
         raise ValueError("cu_seqlens_q needs at least two offsets")
     if p.max_q == 1 and not p.deterministic and p.mask is None:
-        from ._decode import decode
-        return decode(p, out)
+        from ._decode import decode, uses_gqa_kernel
+        if not p.block_scaled or uses_gqa_kernel(p):   # (else the prefill's tiles, before the generic kernel)
+            return decode(p, out)
     if p.max_q == 1 and p.deterministic and p.mask is None:
         done = _fixed_order_decode(p, out)
         if done is not None:
@@ -387,6 +423,8 @@ def solve(p):
             return done
     lse = torch.empty((p.heads, p.tokens), device=p.device, dtype=torch.float32)
     a = build_args(p, out, lse)
+    if p.block_scaled and _fits_prefill(p, out):
+        widen(p, a)
     if _fits_prefill(p, out) and supported(p, "fa_prefill_supported", a):
         # In a mixed chunked-prefill + decode batch the single-query requests
         # take the decode kernel: a 128-row MFMA query tile per head would be

@@ -133,6 +133,11 @@ class BlockAttnArgs(ctypes.Structure):
                 ("k_scale_stride", _arr(_i64, 3)), ("v_scale_stride", _arr(_i64, 3)), ("block", _i64)]
 
 
+class BlockWideArgs(ctypes.Structure):
+    _fields_ = [("size", _i64), ("block", BlockAttnArgs), ("k_wide", _p), ("v_wide", _p), ("capacity", _i64),
+                ("rows", _p), ("flags", _p)]
+
+
 class Rotation(ctypes.Structure):
     _fields_ = [("cos_table", _p), ("sin_table", _p), ("trig_dtype", _i32), ("interleaved", _i32),
                 ("half_rot", _i64), ("table_rows", _i64), ("cos_stride", _arr(_i64, 2)), ("sin_stride", _arr(_i64, 2)),
@@ -188,6 +193,11 @@ def block_attn(a, k_scale, v_scale, block):
         _BLOCK_SIZE, a, _block_tail.pack(k_scale.data_ptr(), v_scale.data_ptr(), *k_scale.stride(), *v_scale.stride(), block))))
 
 
+def block_wide(block, k_wide, v_wide, capacity, rows, flags):
+    """A BlockWideArgs: BlockAttnArgs `block` by way of the workspace at these addresses."""
+    return BlockWideArgs(ctypes.sizeof(BlockWideArgs), block, k_wide, v_wide, capacity, rows, flags)
+
+
 def pack_rotary_rows(*values):
     """A RotaryRowsArgs from its fields' values after `size`."""
     return _pack(RotaryRowsArgs, _rotary_packer, "rotary", (_rotary_packer.size, *values))
@@ -215,6 +225,8 @@ ENTRY_POINTS = {
     "fa_block_decode_fwd": (BlockAttnArgs, ctypes.c_int),
     "fa_block_prefill_supported": (BlockAttnArgs, ctypes.c_int),
     "fa_block_prefill_fwd": (BlockAttnArgs, ctypes.c_int),
+    "fa_block_wide_supported": (BlockWideArgs, ctypes.c_int),
+    "fa_block_wide_fwd": (BlockWideArgs, ctypes.c_int),
     "fa_block_attn_fwd": (BlockAttnArgs, ctypes.c_int),
     "fa_decode_supported": (AttnArgs, ctypes.c_int),
     "fa_decode_fwd": (AttnArgs, ctypes.c_int),

@@ -272,6 +272,18 @@ typedef struct fa_block_attn_args {
   int64_t block;               /* tokens per scale */
 } fa_block_attn_args;
 
+/* The same by way of 16-bit rows: the keys and values that the rows see are
+ * widened to the queries' type into a workspace, and the 16-bit prefill runs on
+ * that (its partials and splits in block.attn). */
+typedef struct fa_block_wide_args {
+  int64_t size;                /* sizeof(fa_block_wide_args) */
+  fa_block_attn_args block;
+  void* k_wide; void* v_wide;  /* [batch, capacity, Hkv, Dqk] / [.., Dv] of the queries' type, 16-byte aligned */
+  int64_t capacity;            /* rows of a request, >= max_seqlen_k */
+  const int32_t* rows;         /* 0, 1, .. batch - 1 */
+  int32_t* flags;              /* [batch, ceil(max_seqlen_k / 64), 2], written by the call */
+} fa_block_wide_args;
+
 /* Two-state merge (out may alias a or b, out_lse may alias a_lse). */
 typedef struct fa_merge_pair_args {
   void* out; const void* a; const void* b;
@@ -372,6 +384,13 @@ int fa_block_decode_fwd(const fa_block_attn_args* args, void* stream);
 int fa_block_prefill_supported(const fa_block_attn_args* args);
 int fa_block_prefill_fwd(const fa_block_attn_args* args, void* stream);
 int fa_block_attn_fwd(const fa_block_attn_args* args, void* stream);
+
+/* Prefill over a block-scaled cache through a 16-bit workspace: what
+ * fa_prefill_fwd takes of 16-bit K/V (head dims that are multiples of 8), rows
+ * of any number; worth its pass over the cache from some hundred query rows per
+ * KV head on. */
+int fa_block_wide_supported(const fa_block_wide_args* args);
+int fa_block_wide_fwd(const fa_block_wide_args* args, void* stream);
 
 int fa_merge_pair(const fa_merge_pair_args* args, void* stream);
 int fa_merge_partials(const fa_merge_partials_args* args, void* stream);

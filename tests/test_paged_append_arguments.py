@@ -223,3 +223,12 @@ def test_attention_refusals(monkeypatch, change, error, match):
 
 def test_attention_takes_block_scales(monkeypatch):
     assert _attend(monkeypatch).block_scaled
+
+
+def test_wide_entry_refuses_null_and_mismatched_arguments():
+    lib = _lib.load()
+    assert lib.fa_block_wide_fwd(None, None) == 1 and not lib.fa_block_wide_supported(None)
+    a = _lib.BlockWideArgs()
+    assert lib.fa_block_wide_fwd(ctypes.byref(a), None) == 1
+    a.size = ctypes.sizeof(a)
+    assert lib.fa_block_wide_fwd(ctypes.byref(a), None) == 1 and not _lib.supported("fa_block_wide_supported", a)
