@@ -17,8 +17,9 @@ struct WideParams {
   fa_block_attn a;
   uint16_t* out[2];       // [batch, capacity, heads, dim], K and V
   int32_t* flags;         // [batch, tiles, 2]: whether a tile may hold values that are not finite
+  int32_t* lengths;       // [batch]: keys of a request in the workspace
   int64_t capacity;
-  int32_t tiles, bf16;
+  int32_t tiles;
   int32_t chunks[2];      // pieces of a head's row
   uint32_t limit;         // scale bytes above it may leave the 16-bit type's range
 };
@@ -105,7 +106,10 @@ __global__ __launch_bounds__(256) void widen_kernel(const WideParams p) {
     }
   }
   const int any = __syncthreads_or(odd);
-  if (threadIdx.x == 0) p.flags[(b * p.tiles + tile) * 2 + which] = any;
+  if (threadIdx.x != 0) return;
+  p.flags[(b * p.tiles + tile) * 2 + which] = any;
+  // (A length past the caller's max_seqlen_k has no rows here.)
+  if (tile == 0 && which == 0) p.lengths[b] = (int)min((int64_t)r.k_len, p.capacity);
 }
 
 // Rows whose output is not finite, where some tile was flagged: a few workgroups
@@ -169,6 +173,8 @@ fa_attn_args wide_attn(const fa_block_wide_args& w) {
     int64_t* const st = i ? a.v_stride : a.k_stride;
     st[0] = w.capacity * heads * dims[i], st[1] = heads * dims[i], st[2] = dims[i], st[3] = 1;
   }
+  a.seqused_k = w.flags + a.batch * 2 * fa_ceil_div(a.max_seqlen_k, TILE);   // `lengths`
+  a.used_k_stride = 1;
   a.block_table = w.rows;
   a.bt_stride[0] = 1, a.bt_stride[1] = 1;
   return a;
@@ -210,23 +216,22 @@ extern "C" int fa_block_wide_fwd(const fa_block_wide_args* args, void* stream) {
   p.out[0] = (uint16_t*)args->k_wide, p.out[1] = (uint16_t*)args->v_wide;
   p.flags = args->flags;
   p.capacity = args->capacity;
-  p.bf16 = bf16;
+  p.lengths = p.flags + p.a.batch * 2 * fa_ceil_div(p.a.max_seqlen_k, TILE);
+  FA_REQUIRE(p.a.max_seqlen_k >= 1, "%s: max_seqlen_k must be positive", who);
   p.tiles = (int32_t)fa_ceil_div(p.a.max_seqlen_k, TILE);
   p.chunks[0] = (int32_t)(p.a.head_dim_qk / codes), p.chunks[1] = (int32_t)(p.a.head_dim_v / codes);
   // 448 * 2^(e - 127) is finite in the type up to these.
   p.limit = bf16 ? 127 + 118 : 127 + 7;
   hipStream_t s = (hipStream_t)stream;
-  if (p.tiles > 0) {
-    const dim3 grid((unsigned)p.tiles, (unsigned)p.a.batch, 2);
-    void (*kern)(const WideParams) = codes == 16 ? (bf16 ? widen_kernel<true, 16> : widen_kernel<false, 16>)
-                                                 : (bf16 ? widen_kernel<true, 8> : widen_kernel<false, 8>);
-    hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, p);
-    const int launched = fa_check_launch(who);
-    if (launched) return launched;
-  }
+  const dim3 grid((unsigned)p.tiles, (unsigned)p.a.batch, 2);
+  void (*kern)(const WideParams) = codes == 16 ? (bf16 ? widen_kernel<true, 16> : widen_kernel<false, 16>)
+                                               : (bf16 ? widen_kernel<true, 8> : widen_kernel<false, 8>);
+  hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, p);
+  const int launched = fa_check_launch(who);
+  if (launched) return launched;
   const fa_attn_args wide = wide_attn(*args);
   const int ran = fa_prefill_fwd(&wide, stream);
-  if (ran || p.tiles == 0) return ran;
+  if (ran) return ran;
   hipLaunchKernelGGL((bf16 ? again_kernel<true> : again_kernel<false>), dim3(256), dim3(256), 0, s, p);
   return fa_check_launch(who);
 }

@@ -136,36 +136,46 @@ def supported(p, name, a):
 
 
 # A block-scaled prefill runs by way of 16-bit rows (fa_block_wide_fwd) from this
-# many query rows and heads per KV head and request on, while the workspace stays
-# below this size.  The pass over the cache costs 3 bytes a value at 4 TB/s, the
-# E4M3 tiles about half as much again as the 16-bit ones for each row.  Measured (us, tiles
-# / by way of 16-bit rows): WIDE_FIGURES
-_WIDE_ROWS = 640
+# many (query row, head) pairs per KV head and request on, while the workspace
+# stays below _WIDE_BYTES.  The pass over the cache costs 3 bytes a value, the E4M3
+# tiles about half as much again as the 16-bit ones for each row.  GPU us, tiles
+# against 16-bit rows: 16 requests of 8000 keys, 32/8 heads d128, 128 rows (512
+# pairs) 431 / 477, 256 rows 824 / 742, 512 rows 1560 / 1282; 4 of 8000 keys, 8/8,
+# 512 rows 153 / 155, 1024 rows 271 / 241; 2 of 8000, 64/8 d64, 64 rows 69 / 73, 128 rows
+# 109 / 99; 2 of 8000, 16/8 d256, 256 rows 165 / 178, 512 rows 282 / 274.  At 256 dims with a softcap or a
+# window the tiles spill: 4 x 17 rows of 1000 keys, softcap and window 126 / 85,
+# window 101 / 77, softcap 90 / 83; 512 rows 280 / 103, 214 / 97, 139 / 115.
+_WIDE_ROWS = 800
+_WIDE_ROWS_SPILLED = 32
 _WIDE_BYTES = 4 << 30
 
 
-def widen(p, a):
-    """The 16-bit workspace of a block-scaled prefill as p.wide, where it pays or
-    nothing else but the generic kernel takes the call.  Calls with a fixed order
-    stay on the tiles, whose choice does not depend on the batch."""
-    if p.q.dtype not in (torch.float16, torch.bfloat16) or p.deterministic or p.max_k < 1:
-        return
+def takes_prefill(p, a):
+    """Whether the MFMA prefill takes arguments `a` of Problem `p`, by way of
+    16-bit rows (p.wide then holds the workspace) for block-scaled caches where
+    that pays or the tiles do not.  Calls with a fixed order stay on the tiles,
+    whose choice does not depend on the batch."""
+    if not p.block_scaled:
+        return _lib.supported("fa_prefill_supported", a)
     rows, visible = p.tokens / p.batch, p.visible_max
-    shared = rows * (p.heads // p.kv_heads) * visible / min(p.max_k, visible + rows)
-    if shared < _WIDE_ROWS and supported(p, "fa_prefill_supported", a):
-        return
+    spilled = p.dim_qk == 256 and (p.softcap > 0 or tuple(p.window) != (-1, -1))
+    least = min(_WIDE_ROWS, _WIDE_ROWS_SPILLED) if spilled else _WIDE_ROWS
+    pays = rows * (p.heads // p.kv_heads) * visible >= least * min(p.max_k, visible + rows)
+    tiles = not pays and supported(p, "fa_prefill_supported", a)
     keys = p.batch * p.max_k * p.kv_heads
-    if 2 * keys * (p.dim_qk + p.dim_v) > _WIDE_BYTES:
-        return
+    size = 2 * keys * (p.dim_qk + p.dim_v)
+    if tiles or p.deterministic or not 0 < size <= _WIDE_BYTES or p.q.dtype == torch.float8_e4m3fn:
+        return tiles or (pays and supported(p, "fa_prefill_supported", a))
     from .interface import _counting
     identity = _counting.rows(p.batch, p.device)
-    work = torch.empty(keys * (p.dim_qk + p.dim_v), dtype=p.q.dtype, device=p.device)
-    flags = torch.empty(2 * p.batch * -(-p.max_k // 64), dtype=torch.int32, device=p.device)
+    work = torch.empty(size // 2, dtype=p.q.dtype, device=p.device)
+    flags = torch.empty(p.batch * (2 * -(-p.max_k // 64) + 1), dtype=torch.int32, device=p.device)
     p.wide = (work.data_ptr(), work.data_ptr() + 2 * keys * p.dim_qk, p.max_k, identity.data_ptr(), flags.data_ptr())
     if supported(p, "fa_prefill_supported", a):
         p.keep += [identity, work, flags]
-    else:
-        p.wide = None
+        return True
+    p.wide = None
+    return pays and supported(p, "fa_prefill_supported", a)
 
 
 def _fits_prefill(p, out):
@@ -423,9 +433,7 @@ def solve(p):
             return done
     lse = torch.empty((p.heads, p.tokens), device=p.device, dtype=torch.float32)
     a = build_args(p, out, lse)
-    if p.block_scaled and _fits_prefill(p, out):
-        widen(p, a)
-    if _fits_prefill(p, out) and supported(p, "fa_prefill_supported", a):
+    if _fits_prefill(p, out) and takes_prefill(p, a):
         # In a mixed chunked-prefill + decode batch the single-query requests
         # take the decode kernel: a 128-row MFMA query tile per head would be
         # almost empty for them.  Packed self-attention (queries and keys on

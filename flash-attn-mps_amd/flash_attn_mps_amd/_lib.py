@@ -184,6 +184,9 @@ _rotary_packer, _append_packer = _packer(RotaryRowsArgs), _packer(PagedAppendArg
 
 _block_tail = struct.Struct("@PP7q")
 _BLOCK_SIZE = struct.pack("@q", ctypes.sizeof(BlockAttnArgs))
+_wide_tail = struct.Struct("@PPqPP")
+_WIDE_SIZE = struct.pack("@q", ctypes.sizeof(BlockWideArgs))
+assert ctypes.sizeof(BlockWideArgs) == 8 + ctypes.sizeof(BlockAttnArgs) + _wide_tail.size
 assert ctypes.sizeof(BlockAttnArgs) == 8 + ctypes.sizeof(AttnArgs) + _block_tail.size
 
 
@@ -195,7 +198,8 @@ def block_attn(a, k_scale, v_scale, block):
 
 def block_wide(block, k_wide, v_wide, capacity, rows, flags):
     """A BlockWideArgs: BlockAttnArgs `block` by way of the workspace at these addresses."""
-    return BlockWideArgs(ctypes.sizeof(BlockWideArgs), block, k_wide, v_wide, capacity, rows, flags)
+    return BlockWideArgs.from_buffer_copy(b"".join((
+        _WIDE_SIZE, block, _wide_tail.pack(k_wide, v_wide, capacity, rows, flags))))
 
 
 def pack_rotary_rows(*values):

@@ -136,7 +136,7 @@ class Problem:
     splits: int = 0
     deterministic: bool = False
     keep: list = field(default_factory=list)   # temporaries that must outlive the launch
-    wide: Optional[tuple] = None            # a block-scaled prefill's 16-bit workspace (_attention.widen)
+    wide: Optional[tuple] = None            # a block-scaled prefill's 16-bit workspace (_attention.takes_prefill)
 
     # ---- derived sizes
     @property

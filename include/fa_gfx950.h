@@ -281,7 +281,7 @@ typedef struct fa_block_wide_args {
   void* k_wide; void* v_wide;  /* [batch, capacity, Hkv, Dqk] / [.., Dv] of the queries' type, 16-byte aligned */
   int64_t capacity;            /* rows of a request, >= max_seqlen_k */
   const int32_t* rows;         /* 0, 1, .. batch - 1 */
-  int32_t* flags;              /* [batch, ceil(max_seqlen_k / 64), 2], written by the call */
+  int32_t* flags;              /* batch * (2 * ceil(max_seqlen_k / 64) + 1) words, written by the call */
 } fa_block_wide_args;
 
 /* Two-state merge (out may alias a or b, out_lse may alias a_lse). */

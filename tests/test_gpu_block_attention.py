@@ -466,3 +466,13 @@ def test_single_rows_that_the_decode_kernel_leaves(device, dim):
     call.check(device)
     call.check(device, window_size=(40, 0), softcap=5.0)
     call.check(device, s_aux=torch.linspace(-2, 2, 8))
+
+
+def test_wide_length_past_the_callers_maximum(device, wide):
+    """A length past max_seqlen_k: the keys up to it, and the other requests as ever."""
+    call = Call([40, 30], [90, 200], 64, 16, 4, 2, 128)
+    want, _ = call.gpu(device)
+    call.used[1] = 220
+    call.table = torch.nn.functional.pad(call.table, (0, 1), value=0)
+    out, _ = call.gpu(device, max_k=200)
+    assert torch.equal(out[:40], want[:40]) and torch.equal(out[40:], want[40:])
