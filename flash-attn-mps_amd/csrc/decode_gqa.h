@@ -111,6 +111,21 @@ FA_DEV void wait_dma_groups(int n) {
   }
 }
 
+#ifndef FA_GQA_CLUSTER
+#define FA_GQA_CLUSTER 2
+#endif
+constexpr int GQA_CLUSTER = FA_GQA_CLUSTER;
+
+FA_DEV void cluster_heads(int& x, int& w) {
+  constexpr unsigned C = GQA_CLUSTER, GROUP = 8 * C;
+  const unsigned gx = gridDim.x, id = (unsigned)x + gx * (unsigned)w, total = gx * gridDim.y * gridDim.z;
+  const unsigned whole = total / GROUP, in = id - id / GROUP * GROUP;
+  const bool tail = id >= whole * GROUP;
+  const unsigned unit = id / GROUP * 8 + (tail ? in / C : in % 8), slot = tail ? in % C : in / 8;
+  x = (int)(unit % (gx / C) * C + slot);
+  w = (int)(unit / (gx / C));
+}
+
 // One head's row over keys [t0, t1) (E4M3 queries, keys and values), one key
 // per lane and only its own KV head's rows, as the generic kernel does: for
 // workgroups of paired heads whose sums met a NaN, which the zero queries and
@@ -232,11 +247,15 @@ __global__ __launch_bounds__(GQA_THREADS, QF8 || BLOCK ? 2 : 1) void decode_gqa_
   const int gr = (int)(a.heads_q / a.heads_k);   // query heads per KV head
   const int group = PACK * gr;
   const int tiles = (group + nh - 1) / nh;
-  const int kh = blockIdx.x / tiles, t0 = (blockIdx.x % tiles) * nh;
+  int x = blockIdx.x, w = fa_decode::split_slot();
+  if constexpr (BLOCK && EB * D < 128) {
+    if (tiles == 1 && gridDim.x % GQA_CLUSTER == 0) cluster_heads(x, w);
+  }
+  const int kh = x / tiles, t0 = (x % tiles) * nh;
   const int nheads = min(nh, group - t0);
   const int h0 = kh * group + t0;
   const int S = a.num_splits;
-  const fa_decode::SplitItem item = fa_decode::split_item(a, ntok, span);
+  const fa_decode::SplitItem item = fa_decode::split_item(a, ntok, span, w);
   if (!item.ok) return;
   const int split = item.split;
   const int64_t b = item.b;

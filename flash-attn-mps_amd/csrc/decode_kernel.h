@@ -273,20 +273,21 @@ FA_DEV RequestInfo request_from_lane(const RequestInfo& r, int l) {
   return o;
 }
 
-FA_DEV SplitItem split_item(const fa_attn_args& a, int rows, int span) {
+FA_DEV int split_slot() { return (int)(blockIdx.y + gridDim.y * blockIdx.z); }
+
+FA_DEV SplitItem split_item(const fa_attn_args& a, int rows, int span, int w) {
   const int S = a.num_splits;
   SplitItem it;
   it.ok = false;
   it.b = 0;
   it.split = 0;
   if (a.batch > 64 * SPLIT_ORDER_CHUNKS) {
-    it.split = blockIdx.y;
-    it.b = blockIdx.z;
+    it.split = w % (int)gridDim.y;
+    it.b = w / (int)gridDim.y;
     it.r = load_request(a, it.b);
     it.ok = it.r.q_len >= 1 && it.r.q_len <= rows;
     return it;
   }
-  const int w = (int)(blockIdx.y + gridDim.y * blockIdx.z);
   const int lane = threadIdx.x & 63;
   const int B = (int)a.batch, nc = (B + 63) / 64;
   RequestInfo rq[SPLIT_ORDER_CHUNKS];
@@ -402,7 +403,7 @@ __global__ __launch_bounds__(DEC_THREADS, FA_DEC_MINB) void decode_kernel(const 
   // before computing the current one).
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, rg = lane >> 4, l16 = lane & 15;
-  const SplitItem item = split_item(a, 1, span);
+  const SplitItem item = split_item(a, 1, span, split_slot());
   if (!item.ok) return;
   const int split = item.split;
   const int64_t b = item.b;
