@@ -362,9 +362,9 @@ def _mixed_batch(p, a, fixed_order=False):
     dec.max_seqlen_q = 1   # the decode kernel takes the one-row requests only
     if not supported(p, "fa_decode_supported", dec):
         return False
-    from ._decode import decode_workgroups, split_plan
+    from ._decode import block_split_plan, decode_workgroups, split_plan
     groups = decode_workgroups(p, 1)
-    splits, span = split_plan(p.batch, groups, p.max_k, 1 if fixed_order else 0)
+    splits, span = (block_split_plan if p.block_scaled else split_plan)(p.batch, groups, p.max_k, 1 if fixed_order else 0)
     dec.num_splits, dec.split_span = splits, span
     if splits > 1:
         _partials(p, dec, (p.batch, splits, p.heads, p.dim_v), (p.batch, p.heads, splits))

@@ -46,3 +46,17 @@ def test_key_splits_follow_the_keys_there_are(rows, heads, dim, batch):
             assert span >= 1 and keys // span >= splits
             taken.append(max(1, min(600 // span, splits)))
     assert (taken or batch == 3) and (rows < 512 or not taken or taken[-1] == 1)
+
+
+@pytest.mark.parametrize("batch", [1, 3, 16, 64, 300])
+@pytest.mark.parametrize("groups", [1, 4, 8, 40])
+@pytest.mark.parametrize("visible", [1, 31, 128, 700, 4099, 20000, 200000])
+def test_block_plan_covers_the_keys_in_even_splits(batch, groups, visible):
+    """Every visible key lies in a split, no split is empty, and spans are whole stages of 32 keys."""
+    from flash_attn_mps_amd._decode import block_split_plan
+    splits, span = block_split_plan(batch, groups, visible, 0)
+    assert splits >= 1 and span % 32 == 0 and splits * span >= visible > (splits - 1) * span
+    assert splits == 1 or span >= 128 or visible < 256
+    for asked in (1, 3):
+        given, span = block_split_plan(batch, groups, visible, asked)
+        assert given <= asked and given * span >= visible
