@@ -12,6 +12,10 @@
 namespace {
 
 constexpr int TILE = 64;   // keys of a workgroup
+// Codes of a thread's piece: 8 are read at once, 16 bytes written next to its
+// neighbour's (16 codes, whose two writes interleave with the neighbours',
+// made the pass 15-20 us of 75 slower: 16 prompts of 256..4096, 16/8 heads d128).
+constexpr int CODES = 8;
 
 struct WideParams {
   fa_block_attn a;
@@ -40,20 +44,20 @@ FA_DEV u32x2 widen4(uint32_t w, float scale) {
                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, true))};
 }
 
-// The first key of request r that some query row sees, down to a multiple of 128.
+// The first key of request r that some query row sees.
 FA_DEV int first_key(const fa_attn_args& a, const RequestInfo& r) {
   if (a.mask_kind != 0 || a.window_left < 0) return 0;
-  return max(r.k_len - r.q_len - a.window_left, 0) & ~127;
+  return max(r.k_len - r.q_len - a.window_left, 0);
 }
 
 FA_DEV bool runs_here(const fa_attn_args& a, const RequestInfo& r) {
   return r.q_len > 1 || (r.q_len == 1 && !(a.flags & FA_FLAG_SKIP_SINGLE_QUERY));
 }
 
-// One workgroup per (tile, request, K or V).  A piece is CODES codes of one row
-// of one head.
-template <bool BF16, int CODES>
+// One workgroup per (tile, request, K or V).
+template <bool BF16>
 __global__ __launch_bounds__(256) void widen_kernel(const WideParams p) {
+  __shared__ int64_t code_at[TILE], scale_at[TILE];
   const fa_block_attn& a = p.a;
   const int tile = blockIdx.x, which = blockIdx.z;
   const int64_t b = blockIdx.y;
@@ -63,44 +67,53 @@ __global__ __launch_bounds__(256) void widen_kernel(const WideParams p) {
   const uint8_t* const in = (const uint8_t*)(which ? a.v : a.k);
   const int begin = tile * TILE, end = min(begin + TILE, (int)min((int64_t)r.k_len, p.capacity));
   bool odd = false;
-  if (runs_here(a, r) && begin >= first_key(a, r) && begin < end) {
-    const int items = (end - begin) * per_key;
-    const uint32_t size = (uint32_t)a.page_size;
+  // The prefill reads whole tiles of up to 128 keys: the first one's keys that no
+  // row sees are zeros here, and their pages are not read.
+  const int first = first_key(a, r);
+  if (runs_here(a, r) && begin >= (first & ~127) && begin < end) {
+    // Where each key's row and scales start, once for all its pieces.
+    const int keys = end - begin;
+    if ((int)threadIdx.x < keys && begin + (int)threadIdx.x >= first) {
+      const uint32_t size = (uint32_t)a.page_size, pos = (uint32_t)begin + threadIdx.x, column = pos / size, row = pos - column * size;
+      const int64_t page = a.block_table[b * a.bt_stride[0] + (int64_t)column * a.bt_stride[1]];
+      const int64_t* const ss = a.scale_stride[which];
+      code_at[threadIdx.x] = page * st[0] + (int64_t)row * st[1];
+      scale_at[threadIdx.x] = page * ss[0] + (int64_t)(row / (uint32_t)a.block) * ss[1];
+    }
+    __syncthreads();
+    // A thread keeps its piece (head h, chunk c) over the keys.
+    const int span = per_key < 256 ? per_key : 256, step = 256 / span;   // threads of a key, keys at once
+    const int key0 = (int)threadIdx.x / span, mine = key0 < step ? (int)threadIdx.x - key0 * span : per_key;
     uint16_t* const out = p.out[which] + (b * p.capacity + begin) * per_key * CODES;
-    constexpr int N = 4;   // pieces of a thread in flight
-    for (int i0 = threadIdx.x; i0 < items; i0 += N * 256) {
-      uint32_t w[N][CODES / 4], e[N];
+    const int64_t head_codes = st[2], head_scales = a.scale_stride[which][2];
+    for (int piece = mine; piece < per_key; piece += 256) {
+      const int h = piece / chunks;
+      const uint8_t* const codes = in + h * head_codes + (piece - h * chunks) * CODES;
+      const uint8_t* const scales = a.scale[which] + h * head_scales;
+      constexpr int N = 4;   // keys of a thread in flight
+      for (int k0 = key0; k0 < keys; k0 += N * step) {
+        u32x2 w[N];
+        uint32_t e[N];
 #pragma unroll
-      for (int n = 0; n < N; ++n) {
-        const int i = i0 + n * 256;
-        if (i >= items) continue;
-        const uint32_t key = (uint32_t)i / (uint32_t)per_key, rem = (uint32_t)i - key * (uint32_t)per_key;
-        const uint32_t h = rem / (uint32_t)chunks, c = rem - h * (uint32_t)chunks;
-        const uint32_t pos = (uint32_t)begin + key, column = pos / size, row = pos - column * size;
-        const int64_t page = a.block_table[b * a.bt_stride[0] + (int64_t)column * a.bt_stride[1]];
-        const uint8_t* const src = in + page * st[0] + (int64_t)row * st[1] + (int64_t)h * st[2] + c * CODES;
-        if constexpr (CODES == 16) {
-          const u32x4 v = *(const u32x4*)src;
-          w[n][0] = v[0], w[n][1] = v[1], w[n][2] = v[2], w[n][3] = v[3];
-        } else {
-          const u32x2 v = *(const u32x2*)src;
-          w[n][0] = v[0], w[n][1] = v[1];
+        for (int n = 0; n < N; ++n) {
+          const int key = k0 + n * step;
+          w[n] = u32x2{0, 0};
+          e[n] = 127;
+          if (key >= keys || begin + key < first) continue;
+          const uint8_t* const src = codes + code_at[key];
+          w[n] = *(const u32x2*)src;
+          e[n] = scales[scale_at[key]];
         }
-        e[n] = scale_byte(a, which, page, (int)row, (int)h);
-      }
 #pragma unroll
-      for (int n = 0; n < N; ++n) {
-        const int i = i0 + n * 256;
-        if (i >= items) continue;
-        const float scale = e8m0_to_f32(e[n]);
-        odd |= e[n] > p.limit;
-        u32x4* const dst = (u32x4*)(out + (int64_t)i * CODES);
-#pragma unroll
-        for (int k = 0; k < CODES / 4; k += 2) {
-          const u32x2 x = widen4<BF16>(w[n][k], scale), y = widen4<BF16>(w[n][k + 1], scale);
-          dst[k / 2] = u32x4{x[0], x[1], y[0], y[1]};
+        for (int n = 0; n < N; ++n) {
+          const int key = k0 + n * step;
+          if (key >= keys) continue;
+          const float scale = e8m0_to_f32(e[n]);
+          odd |= e[n] > p.limit;
+          const u32x2 x = widen4<BF16>(w[n][0], scale), y = widen4<BF16>(w[n][1], scale);
+          *(u32x4*)(out + ((int64_t)key * per_key + piece) * CODES) = u32x4{x[0], x[1], y[0], y[1]};
           // NaN codes: 0x7f without the sign.
-          odd |= ((((w[n][k] & 0x7f7f7f7fu) + 0x01010101u) | ((w[n][k + 1] & 0x7f7f7f7fu) + 0x01010101u)) & 0x80808080u) != 0;
+          odd |= ((((w[n][0] & 0x7f7f7f7fu) + 0x01010101u) | ((w[n][1] & 0x7f7f7f7fu) + 0x01010101u)) & 0x80808080u) != 0;
         }
       }
     }
@@ -148,16 +161,12 @@ __global__ __launch_bounds__(256) void again_kernel(const WideParams p) {
   }
 }
 
-// Codes of a piece: 16, or 8 where dims or strides ask for it; 0 where the rows
-// have no aligned pieces.
-int piece_codes(const fa_attn_args& a) {
-  for (int codes : {16, 8}) {
-    bool ok = a.head_dim_qk % codes == 0 && a.head_dim_v % codes == 0 && a.k_stride[3] == 1 && a.v_stride[3] == 1 &&
-              (uintptr_t)a.k % codes == 0 && (uintptr_t)a.v % codes == 0;
-    for (int i = 0; i < 3; ++i) ok = ok && a.k_stride[i] % codes == 0 && a.v_stride[i] % codes == 0;
-    if (ok) return codes;
-  }
-  return 0;
+// Whether the rows come in aligned pieces.
+bool pieces_aligned(const fa_attn_args& a) {
+  bool ok = a.head_dim_qk % CODES == 0 && a.head_dim_v % CODES == 0 && a.k_stride[3] == 1 && a.v_stride[3] == 1 &&
+            (uintptr_t)a.k % CODES == 0 && (uintptr_t)a.v % CODES == 0;
+  for (int i = 0; i < 3; ++i) ok = ok && a.k_stride[i] % CODES == 0 && a.v_stride[i] % CODES == 0;
+  return ok;
 }
 
 // The 16-bit call on the workspace: request b's keys are page b of pages of
@@ -184,7 +193,7 @@ bool wide_ok(const fa_block_wide_args* w, fa_block_attn* a) {
   if (!w || w->size != (int64_t)sizeof(fa_block_wide_args) || !fa_block_arguments(&w->block, a)) return false;
   if ((a->q_dtype != FA_BF16 && a->q_dtype != FA_F16) || a->out_dtype != a->q_dtype) return false;
   if (a->head_dim_v > 256 || a->batch > 65535 || a->max_seqlen_k > w->capacity || w->capacity > INT32_MAX / 2) return false;
-  if (w->capacity < 1 || !piece_codes(*a)) return false;
+  if (w->capacity < 1 || !pieces_aligned(*a)) return false;
   // (Rows of a wave's output are read back as they were written.)
   if (a->out_stride[2] != 1) return false;
   const fa_attn_args wide = wide_attn(*w);
@@ -212,21 +221,18 @@ extern "C" int fa_block_wide_fwd(const fa_block_wide_args* args, void* stream) {
   }
   if (p.a.total_q == 0) return FA_OK;
   const bool bf16 = p.a.q_dtype == FA_BF16;
-  const int codes = piece_codes(p.a);
   p.out[0] = (uint16_t*)args->k_wide, p.out[1] = (uint16_t*)args->v_wide;
   p.flags = args->flags;
   p.capacity = args->capacity;
   p.lengths = p.flags + p.a.batch * 2 * fa_ceil_div(p.a.max_seqlen_k, TILE);
   FA_REQUIRE(p.a.max_seqlen_k >= 1, "%s: max_seqlen_k must be positive", who);
   p.tiles = (int32_t)fa_ceil_div(p.a.max_seqlen_k, TILE);
-  p.chunks[0] = (int32_t)(p.a.head_dim_qk / codes), p.chunks[1] = (int32_t)(p.a.head_dim_v / codes);
+  p.chunks[0] = (int32_t)(p.a.head_dim_qk / CODES), p.chunks[1] = (int32_t)(p.a.head_dim_v / CODES);
   // 448 * 2^(e - 127) is finite in the type up to these.
   p.limit = bf16 ? 127 + 118 : 127 + 7;
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid((unsigned)p.tiles, (unsigned)p.a.batch, 2);
-  void (*kern)(const WideParams) = codes == 16 ? (bf16 ? widen_kernel<true, 16> : widen_kernel<false, 16>)
-                                               : (bf16 ? widen_kernel<true, 8> : widen_kernel<false, 8>);
-  hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, p);
+  hipLaunchKernelGGL((bf16 ? widen_kernel<true> : widen_kernel<false>), grid, dim3(256), 0, s, p);
   const int launched = fa_check_launch(who);
   if (launched) return launched;
   const fa_attn_args wide = wide_attn(*args);

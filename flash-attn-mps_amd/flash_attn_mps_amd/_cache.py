@@ -17,6 +17,7 @@ flash_attn_mps/_cache.py:55-155).
   input's bits.
 """
 import ctypes
+import operator
 from functools import lru_cache
 
 import torch
@@ -289,7 +290,11 @@ def _pair_axis_words(pair_axes, half, axes):
         if axes > 1:
             raise ValueError(f"positions on {axes} axes need pair_axes, the axis of each of the {half} rotated pairs")
         return (0,) * 8
-    if len(pair_axes) != half or any(type(a) is not int or not 0 <= a < axes for a in pair_axes):
+    try:
+        pair_axes = [operator.index(a) for a in pair_axes]
+    except TypeError:
+        pair_axes = []
+    if len(pair_axes) != half or any(not 0 <= a < axes for a in pair_axes):
         raise ValueError(f"pair_axes must hold one axis in 0..{axes - 1} for each of the {half} rotated pairs")
     words = [0] * 8
     for i, a in enumerate(pair_axes):
@@ -310,6 +315,8 @@ def _rotation(cos, sin, positions, pair_axes, interleaved, tokens, dims, device)
     if cos.device != device or sin.device != device:
         raise ValueError(f"rotary tables on {cos.device} / {sin.device}; expected {device}")
     rows, half = cos.shape
+    if half < 1 or rows < 1:
+        raise ValueError(f"rotary tables {tuple(cos.shape)} hold no position or no pair")
     if 2 * half > min(dims):
         raise ValueError(f"rotary_dim {2 * half} exceeds the head dim {min(dims)}")
     axes, at = 1, (0, 0, 1, 0, 0)

@@ -476,3 +476,19 @@ def test_wide_length_past_the_callers_maximum(device, wide):
     call.table = torch.nn.functional.pad(call.table, (0, 1), value=0)
     out, _ = call.gpu(device, max_k=200)
     assert torch.equal(out[:40], want[:40]) and torch.equal(out[40:], want[40:])
+
+
+def test_wide_keys_before_every_window_are_not_read(device, wide):
+    """Pages and scales that hold NaN before the first row's window change no bit."""
+    for dim, rows in ((128, 40), (256, 40), (64, 200)):
+        call = Call([rows, rows], [700 + rows, 300 + rows], 64, 16, 8, 2, dim)
+        want, want_lse = call.gpu(device, window_size=(77, 0))
+        for b, length in enumerate((700, 300)):
+            for page in call.table[b, :(length - 77) // 64].tolist():
+                for t in (call.k, call.v, call.ks, call.vs):
+                    t.view(torch.uint8)[page] = 255
+            edge = int(call.table[b, (length - 77) // 64])
+            for t in (call.k, call.v):
+                t.view(torch.uint8)[edge, :(length - 77) % 64] = 0x7f
+        out, lse = call.gpu(device, window_size=(77, 0))
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)

@@ -65,6 +65,9 @@ ROWS = torch.zeros(6, 2, 64, dtype=torch.float16)
     (dict(pair_axes=[0] * 31), ValueError, "pair_axes"),
     (dict(pair_axes=[True] * 32), ValueError, "pair_axes"),
     (dict(pair_axes=torch.zeros(32)), TypeError, "host"),
+    (dict(pair_axes=[0.5] * 32), ValueError, "pair_axes"),
+    (dict(rotary_cos=torch.zeros(9, 0), rotary_sin=torch.zeros(9, 0)), ValueError, "no position or no pair"),
+    (dict(rotary_cos=torch.zeros(0, 32), rotary_sin=torch.zeros(0, 32)), ValueError, "no position or no pair"),
     (dict(rotary_sin=torch.zeros(9, 31)), ValueError, "rotary_sin"),
     (dict(rotary_cos=torch.zeros(9, 33), rotary_sin=torch.zeros(9, 33)), ValueError, "head dim"),
     (dict(rotary_cos=torch.zeros(9, 32, dtype=torch.float64), rotary_sin=torch.zeros(9, 32, dtype=torch.float64)), TypeError, "tables"),
