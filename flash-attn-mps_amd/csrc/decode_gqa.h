@@ -111,10 +111,13 @@ FA_DEV void wait_dma_groups(int n) {
   }
 }
 
-#ifndef FA_GQA_CLUSTER
-#define FA_GQA_CLUSTER 2
-#endif
-constexpr int GQA_CLUSTER = FA_GQA_CLUSTER;
+// BLOCK with slot rows of 64 bytes, half a cache line: two KV heads read each
+// line, so the workgroups of neighbouring heads run on one XCD, eight dispatches
+// apart (workgroups are dealt to the 8 XCDs in turn), and the second finds the
+// line in that XCD's L2.  32 requests x 4 rows of up to 12000 keys, 64/8 heads
+// d64: 90.6 -> 69.0 us, behind a window of 4095 65.2 -> 56.2; clusters of 4 gain
+// nothing more.  The last dispatches, fewer than a whole round, stay in order.
+constexpr int GQA_CLUSTER = 2;
 
 FA_DEV void cluster_heads(int& x, int& w) {
   constexpr unsigned C = GQA_CLUSTER, GROUP = 8 * C;
@@ -208,9 +211,13 @@ FA_DEV void e4m3_row(const fa_attn_args& a, int64_t b, const RequestInfo& r, int
 // lane and handed over by v_readlane.  K's multiplies the scores in fp32, V's
 // enters the widening conversion, which takes a power of two for nothing; so the
 // loop has the E4M3 kernel's arithmetic.  A column whose sum is not finite runs
-// again by block_row, which reads only what a row sees.
+// again by block_row, which reads only what a row sees.  HBM bounds long contexts
+// (64 requests of 16K keys on average, 32/8 heads d128, 2.09 GB: 365 us, 5.7 TB/s) and
+// a workgroup's first loads, a chain of lengths, table, then rows, short ones.
+// 64-dim heads ask for four waves per SIMD, two registers short of what they would
+// take: 32 x 4 rows, 64/8 heads d64 75.7 -> 70.0 us, behind a window 55.7 -> 50.9.
 template <typename T, int D, bool CAP, typename KT = T, int PACK = 1, bool QF8 = false, bool BLOCK = false>
-__global__ __launch_bounds__(GQA_THREADS, QF8 || BLOCK ? 2 : 1) void decode_gqa_kernel(const typename AttnArgsOf<BLOCK>::type a,
+__global__ __launch_bounds__(GQA_THREADS, BLOCK && D / PACK == 64 ? 4 : QF8 || BLOCK ? 2 : 1) void decode_gqa_kernel(const typename AttnArgsOf<BLOCK>::type a,
                                                                              const int span) {
   static_assert(D == 64 || D == 128 || D == 256, "rows of 64, 128 or 256 elements");
   static_assert((PACK == 1 && D <= 128) || (PACK == 2 && (D == 128 || (D == 256 && KT::id == FA_E4M3))),
