@@ -343,8 +343,11 @@ FA_DEV auto lane_offset(int h, int64_t head_stride, int e, int64_t stride) {
 }
 
 // Passes of a wave over a token's rows whose loads are all issued before the
-// first of them is used.
-constexpr int BATCH = 2;
+// first of them is used.  GPU us with 1 / 2 / 3 / 4 / 6 / 8: 9001 tokens of 16 + 16
+// heads d80, two axes (94 MB) 32.4 / 31.5 / 30.4 / 28.8 / 32.7 / 33.2; 4100 rows of
+// 16 + 4 + 4 heads d256 to a 16-bit cache (103 MB) 26.4 / 26.6 / 26.9 / 26.4 / 25.3 /
+// 25.4 (registers, and so waves, are what more of them cost).
+constexpr int BATCH = 4;
 
 template <typename XT, typename TT, int CACHE, bool POS, int W>
 FA_DEV void token_rows(const AppendParams& p, uint32_t w, int lane) {
