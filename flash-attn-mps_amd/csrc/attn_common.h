@@ -82,6 +82,13 @@ FA_DEV float e8m0_to_f32(uint32_t e) {
   return __uint_as_float(e == 0 ? 0x00400000u : e == 255 ? 0x7fc00000u : e << 23);
 }
 
+// The largest scale byte under which every code is finite in T, and the byte as the
+// kernels that widen to T take it: NaN past that, so that every row that meets such
+// a block runs again in fp32.  (An infinity would not always show: times a
+// negative query it is a probability of zero.)
+template <typename T> constexpr uint32_t widest_scale() { return T::id == FA_BF16 ? 127 + 119 : 127 + 7; }
+template <typename T> FA_DEV uint32_t scale_for(uint32_t e) { return e > widest_scale<T>() ? 255u : e; }
+
 // Scale byte of head kh for the key at row `row` of page `page` (V: which = 1).
 FA_DEV uint32_t scale_byte(const fa_block_attn& a, int which, int64_t page, int row, int kh) {
   const int64_t* st = a.scale_stride[which];

@@ -429,7 +429,7 @@ __global__ __launch_bounds__(GQA_THREADS, BLOCK && D / PACK == 64 ? 4 : QF8 || B
 #pragma unroll
         for (int u = 0; u < PACK; ++u)
           w |= scale_byte(a, 0, pages, row, PACK * kh + u) << (8 * u) |
-               scale_byte(a, 1, pages, row, PACK * kh + u) << (16 + 8 * u);
+               scale_for<T>(scale_byte(a, 1, pages, row, PACK * kh + u)) << (16 + 8 * u);
       }
       if (ch & 1) scales_odd = w;
       else scales_even = w;

@@ -443,6 +443,33 @@ def test_wide_not_finite(device, wide):
     assert (out.cpu()[~small].abs() >= 5.9e4).all()
 
 
+def beyond_16_bits(device, rows, dtype):
+    """One key, then one value, past the 16-bit type's range.  The key meets a small negative
+    query: its score is -0.6, where an infinity in its place would leave it out unseen."""
+    byte = 127 + (10 if dtype == torch.float16 else 120)     # 448 * 2^10 = 458752; 448 * 2^120 = 1.75 * 2^128
+    for which in ("k", "v")[dtype == torch.bfloat16:]:
+        call = Call([rows, 1], [200, 30], 64, 16, 4, 2, 128, dtype)
+        codes, scales = (call.k, call.ks) if which == "k" else (call.v, call.vs)
+        page = int(call.table[0, 0])
+        codes.view(torch.uint8)[page, 16:32, 1] = 0
+        codes.view(torch.uint8)[page, 20, 1, 7] = 0x7e
+        scales.view(torch.uint8)[page, 1, 1] = byte
+        call.q[:, 2:, 7] = -2.0 ** -16
+        call.check(device)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows", [1, 3, 70])
+def test_keys_and_values_beyond_16_bits(device, rows, dtype):
+    beyond_16_bits(device, rows, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_wide_keys_and_values_beyond_16_bits(device, wide, dtype):
+    beyond_16_bits(device, 70, dtype)
+    assert "fa_block_wide_fwd" in wide
+
+
 def test_wide_layouts_and_replays(device, wide):
     test_strided_caches(device)
     test_empty_requests_and_padding(device)
