@@ -10,9 +10,9 @@
 // small ones.
 //
 // A unit is W pairs of a row (W = 16 bytes of elements, or one pair where
-// strides, dims or alignment, of the tables too, forbid vectors): two pieces of W elements, next to
-// each other for interleaved pairs, half_rot apart otherwise; dims that do not
-// rotate are copied two pieces a unit.  A lane keeps its unit over all the
+// strides, dims or alignment, of the tables too, forbid vectors): two pieces of W
+// elements, next to each other for interleaved pairs, half_rot apart otherwise;
+// dims that do not rotate are copied two pieces a unit.  A lane keeps its unit over all the
 // heads it takes, so cos and sin are loaded once per token and lane.  A wave
 // works on one token, or on one block of one head: what follows from those
 // (request, position, page) is scalar.
@@ -23,6 +23,11 @@
 // result does not depend on any order.  The rows stay in registers until the scale
 // is known, and are turned a second time (16 registers a row would hold them
 // turned, 8 do as they came).
+//
+// Kernel times: 9001 tokens of 16 + 16 heads d80 on two axes, 94 MB: 26.6 us, 3.5
+// TB/s; 4100 rows of 16 + 4 + 4 heads d256 to a 16-bit cache, 103 MB: 23.6 us, 4.4
+// TB/s; 36K rows of 16 + 8 + 8 heads d128 to a block-scaled one, 619 MB: 147 us, 4.2
+// TB/s (a large copy: 4.8); one token: 4.0 us, with its append 5.9.
 #include "attn_common.h"
 
 namespace {
@@ -446,7 +451,9 @@ FA_DEV int block_exponent(float most) {
   return max(e, -100);
 }
 
-// Rows a lane holds between a block's largest magnitude and its codes.
+// Rows a lane holds between a block's largest magnitude and its codes.  GPU us with
+// 2 / 4 / 8: 36K rows, blocks of 32, 157.4 / 147.4 / 146.3; 64 requests of one row,
+// blocks of 16, 5.7 / 5.7 / 6.3.
 constexpr int HOLD = 4;
 
 template <typename XT, typename TT, bool POS, int W>
@@ -722,7 +729,9 @@ int run_append(AppendParams& p, int dtype, int cache, void* stream, const char* 
   }
   // A few tokens: every pass over a token's rows on a wave of its own, for the
   // shortest chain.  Many: a wave a token, which finds its request, position and
-  // cos/sin once.
+  // cos/sin once.  GPU us, a wave each / a wave a token: one token of 32 + 8 heads
+  // d128 3.5 / 5.8; 9001 tokens of 16 + 16 heads d80 39.7 / 26.8; up to 32768 waves
+  // neither side gains.
   p.token_waves = (uint32_t)(passes > 0 && p.tokens * passes <= 4096 ? passes : 1);
   FA_REQUIRE(p.tokens * p.token_waves <= INT32_MAX, "%s: too many rows", who);
   p.threads = THREADS;

@@ -141,9 +141,9 @@ def supported(p, name, a):
 # tiles about half as much again as the 16-bit ones for each row.  GPU us, tiles
 # against 16-bit rows: 16 requests of 8000 keys, 32/8 heads d128, 128 rows (512
 # pairs) 431 / 477, 256 rows 824 / 742, 512 rows 1560 / 1282; 4 of 8000 keys, 8/8,
-# 512 rows 153 / 155, 1024 rows 271 / 241; 2 of 8000, 64/8 d64, 64 rows 69 / 73, 128 rows
-# 109 / 99; 2 of 8000, 16/8 d256, 256 rows 165 / 178, 512 rows 282 / 274.  At 256 dims with a softcap or a
-# window the tiles spill: 4 x 17 rows of 1000 keys, softcap and window 126 / 85,
+# 512 rows 153 / 155, 1024 rows 271 / 241; 2 of 8000, 64/8 d64, 64 rows 69 / 73,
+# 128 rows 109 / 99; 2 of 8000, 16/8 d256, 256 rows 165 / 178, 512 rows 282 / 274.
+# At 256 dims with a softcap or a window the tiles spill: 4 x 17 rows of 1000 keys, softcap and window 126 / 85,
 # window 101 / 77, softcap 90 / 83; 512 rows 280 / 103, 214 / 97, 139 / 115.
 _WIDE_ROWS = 800
 _WIDE_ROWS_SPILLED = 32

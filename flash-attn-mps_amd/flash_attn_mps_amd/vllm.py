@@ -74,7 +74,8 @@ def flash_attn_varlen_func(
 
     ``k_descale`` / ``v_descale`` are float32 [B, Hkv], or, for a paged E4M3 cache as
     ``append_paged_kvcache`` fills it, float8_e8m0fnu [pages, page_size / block, Hkv]:
-    a power of two per block of tokens and head, in place of descales.
+    a power of two per block of tokens and head, in place of descales.  With float16
+    queries the cache's values enter products as float16 (below 2^-25 as zeros).
     """
     reject_training(dropout_p, return_attn_probs, (q, k, v))
     if fa_version not in (2, 3, 4):

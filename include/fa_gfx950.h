@@ -262,8 +262,9 @@ typedef struct fa_attn_args {
  * [pages, P, Hkv, D], and rows j * block .. of a page carry one power of two per
  * head, the E8M0 byte e at k_scale[page * stride[0] + j * stride[1] + head *
  * stride[2]] (j < P / block, `block` dividing P): a value is code * 2^(e - 127),
- * NaN with e = 255.  attn.k_descale / v_descale are NULL, attn.q is any input type.  No counterpart in the
- * reference, whose FP8 caches have one scale per request and head. */
+ * NaN with e = 255.  attn.k_descale / v_descale are NULL, attn.q is any input
+ * type.  No counterpart in the reference, whose FP8 caches have one scale per
+ * request and head. */
 typedef struct fa_block_attn_args {
   int64_t size;                /* sizeof(fa_block_attn_args) */
   fa_attn_args attn;
