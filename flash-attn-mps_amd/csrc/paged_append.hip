@@ -26,7 +26,7 @@
 //
 // Kernel times: 9001 tokens of 16 + 16 heads d80 on two axes, 94 MB: 26.6 us, 3.5
 // TB/s; 4100 rows of 16 + 4 + 4 heads d256 to a 16-bit cache, 103 MB: 23.6 us, 4.4
-// TB/s; 36K rows of 16 + 8 + 8 heads d128 to a block-scaled one, 619 MB: 147 us, 4.2
+// TB/s; 36K rows of 16 + 8 + 8 heads d128 to a block-scaled one, 619 MB: 150 us, 4.1
 // TB/s (a large copy: 4.8); one token: 4.0 us, with its append 5.9.
 #include "attn_common.h"
 
@@ -270,25 +270,35 @@ FA_DEV Piece<W> narrow(const float (&f)[W]) {
   }
 }
 
+// a x - b y.  TIES: the rounding of b y goes back in (a large number where
+// there is none, b y being infinite), since ties between E4M3 codes are where
+// rounding twice shows: of 20M rotated values 14 codes off the 64-bit ones, 20
+// without it and 32 with each product rounded.
+template <bool TIES>
+FA_DEV float turned_by(float a, float x, float b, float y) {
+  const float by = b * y, v = fmaf(a, x, -by);
+  return TIES ? v + fminf(fmaf(-b, y, by), 3e38f) : v;
+}
+
 // The W pairs of a unit turned; lo and hi are its pieces.
-template <int W>
+template <bool TIES, int W>
 FA_DEV void turn(float (&lo)[W], float (&hi)[W], const float (&c)[W], const float (&s)[W], bool interleaved) {
   if (W > 1 && interleaved) {
 #pragma unroll
     for (int j = 0; j < W; j += 2) {
       const float a = lo[j], b = lo[j + 1], x = hi[j], y = hi[j + 1];
       const int m = j / 2, n = (W + j) / 2;
-      lo[j] = fmaf(a, c[m], -(b * s[m]));
-      lo[j + 1] = fmaf(b, c[m], a * s[m]);
-      hi[j] = fmaf(x, c[n], -(y * s[n]));
-      hi[j + 1] = fmaf(y, c[n], x * s[n]);
+      lo[j] = turned_by<TIES>(a, c[m], b, s[m]);
+      lo[j + 1] = turned_by<TIES>(b, c[m], -a, s[m]);
+      hi[j] = turned_by<TIES>(x, c[n], y, s[n]);
+      hi[j + 1] = turned_by<TIES>(y, c[n], -x, s[n]);
     }
   } else {
 #pragma unroll
     for (int j = 0; j < W; ++j) {
       const float a = lo[j], b = hi[j];
-      lo[j] = fmaf(a, c[j], -(b * s[j]));
-      hi[j] = fmaf(b, c[j], a * s[j]);
+      lo[j] = turned_by<TIES>(a, c[j], b, s[j]);
+      hi[j] = turned_by<TIES>(b, c[j], -a, s[j]);
     }
   }
 }
@@ -423,7 +433,7 @@ FA_DEV void token_rows(const AppendParams& p, uint32_t w, int lane) {
         float f[W], g[W];
         widen<XT, W>(a[k], f);
         widen<XT, W>(z[k], g);
-        if (turns) turn<W>(f, g, c, s, inter);
+        if (turns) turn<CACHE == CACHE_E4M3>(f, g, c, s, inter);
         if (codes) {
           const float scale = r.scale[h * r.scale_stride];
 #pragma unroll
@@ -488,13 +498,13 @@ FA_DEV void own_block(const AppendParams& p, uint32_t group, int lane, uint32_t*
     a = load_piece<XT, W>(src, lane_offset<W>(h, r.xs[1], x.lo, r.xs[2]));
     z = x.hi >= 0 ? load_piece<XT, W>(src, lane_offset<W>(h, r.xs[1], x.hi, r.xs[2])) : Piece<W>{};
   };
-  auto turned = [&](int row, int u, const Unit& x, Piece<W> a, Piece<W> z, float (&f)[W], float (&g)[W]) {
+  auto turned = [&](auto ties, int row, int u, const Unit& x, Piece<W> a, Piece<W> z, float (&f)[W], float (&g)[W]) {
     widen<XT, W>(a, f);
     widen<XT, W>(z, g);
     if (!x.turns) return;
     float c[W], s[W];
     load_trig<TT, POS, W>(p, token + row, base + row, u * W, c, s);
-    turn<W>(f, g, c, s, inter);
+    turn<decltype(ties)::value>(f, g, c, s, inter);
   };
   // The largest finite magnitude (a maximum leaves NaN out; infinities are rare).
   auto largest = [&](float most, const float (&f)[W], const float (&g)[W]) {
@@ -524,7 +534,7 @@ FA_DEV void own_block(const AppendParams& p, uint32_t group, int lane, uint32_t*
     for (int i = 0; i < HOLD; ++i) {
       const int row = first + wave + i * waves;
       if (!on || row >= last) continue;
-      turned(row, u0, x, a[i], z[i], f, g);
+      turned(std::false_type{}, row, u0, x, a[i], z[i], f, g);
       most = largest(most, f, g);
     }
   } else if (on) {
@@ -532,7 +542,7 @@ FA_DEV void own_block(const AppendParams& p, uint32_t group, int lane, uint32_t*
       for (int u = u0; u < r.units; u += p.lanes) {
         const Unit y = unit_of<W>(r, inter, u);
         load(row, y, a[0], z[0]);
-        turned(row, u, y, a[0], z[0], f, g);
+        turned(std::false_type{}, row, u, y, a[0], z[0], f, g);
         most = largest(most, f, g);
       }
   }
@@ -580,7 +590,7 @@ FA_DEV void own_block(const AppendParams& p, uint32_t group, int lane, uint32_t*
     for (int i = 0; i < HOLD; ++i) {
       const int row = first + wave + i * waves;
       if (row >= last) continue;
-      turned(row, u0, x, a[i], z[i], f, g);
+      turned(std::true_type{}, row, u0, x, a[i], z[i], f, g);
       store(row, x, f, g, inverse);
     }
   } else {
@@ -588,7 +598,7 @@ FA_DEV void own_block(const AppendParams& p, uint32_t group, int lane, uint32_t*
       for (int u = u0; u < r.units; u += p.lanes) {
         const Unit y = unit_of<W>(r, inter, u);
         load(row, y, a[0], z[0]);
-        turned(row, u, y, a[0], z[0], f, g);
+        turned(std::true_type{}, row, u, y, a[0], z[0], f, g);
         store(row, y, f, g, inverse);
       }
   }

@@ -242,6 +242,26 @@ def test_block_extremes(device, fill):
         assert torch.equal(torch.signbit(c.cpu().float()), torch.signbit(code)) or fill != fill
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rotated_infinities_saturate(device, interleaved, dtype):
+    """An infinity turns into two, which leave the scale alone and become the largest codes."""
+    x = normal((20, 2, 64), 5, dtype)
+    x[3, 0, 4], x[17, 1, 25], x[9, 0, 60] = float("inf"), -float("inf"), float("inf")
+    codes, scale = random_cache(3, 16, 16, 2, 64, 3)
+    cu, used = torch.tensor([0, 20], dtype=torch.int32), torch.tensor([20], dtype=torch.int32)
+    table, (cos, sin) = torch.tensor([[2, 0]], dtype=torch.int32), tables(20, 16)
+    cache, caches_scale = codes.to(device), scale.to(device)
+    fa.append_paged_kvcache(x.to(device), x.to(device), cache, cache.clone(), cu.to(device), used.to(device), table.to(device),
+                            rotary_cos=cos.to(device), rotary_sin=sin.to(device), rotary_interleaved=interleaved,
+                            k_scale=caches_scale, v_scale=caches_scale.clone())
+    turned = rotate(x, cos, sin, torch.arange(20)[None], None, interleaved)
+    assert turned.isinf().sum() == 5
+    code, factor = append(codes, scale, turned, cu, used, table)
+    assert torch.equal(scale_values(caches_scale), factor)
+    assert_codes(cache, code, False)
+
+
 def test_pages_out_of_reach_are_skipped(device):
     """Pages that are negative or past the cache, positions past the table, lengths below the new rows."""
     for cache in ("block", "same", "head"):
