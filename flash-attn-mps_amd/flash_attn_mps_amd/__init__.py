@@ -64,7 +64,8 @@ def append_paged_kvcache(k, v, k_cache, v_cache, cu_seqlens_q, seqused_k, block_
       tokens and head, written by the append.  A block takes the smallest one >=
       2^-100 under which its largest finite new magnitude is at most 448; if it
       holds earlier rows of its request, the larger of that and its old one, and
-      those rows are coded again.  ``vllm.flash_attn_varlen_func`` reads such a cache.
+      those rows are coded again.  ``vllm.flash_attn_varlen_func`` reads such a
+      cache; let it start as zeros (NaN codes where no row looks cost time).
     """
     from ._cache import append_paged_kvcache as _append
     return _append(k, v, k_cache, v_cache, cu_seqlens_q, seqused_k, block_table, q=q, cos=rotary_cos, sin=rotary_sin,
