@@ -103,14 +103,15 @@ __global__ __launch_bounds__(256) void widen_kernel(const WideParams p) {
           if (key >= keys || begin + key < first) continue;
           const uint8_t* const src = codes + code_at[key];
           w[n] = *(const u32x2*)src;
-          e[n] = scale_for<T>(scales[scale_at[key]]);
+          e[n] = scales[scale_at[key]];
         }
 #pragma unroll
         for (int n = 0; n < N; ++n) {
           const int key = k0 + n * step;
           if (key >= keys) continue;
-          const float scale = e8m0_to_f32(e[n]);
-          odd |= e[n] == 255;
+          const uint32_t byte = scale_for<T>(e[n]);   // (here: the loads above are in flight together)
+          const float scale = e8m0_to_f32(byte);
+          odd |= byte == 255;
           const u32x2 x = widen4<BF16>(w[n][0], scale), y = widen4<BF16>(w[n][1], scale);
           *(u32x4*)(out + ((int64_t)key * per_key + piece) * CODES) = u32x4{x[0], x[1], y[0], y[1]};
           // NaN codes: 0x7f without the sign.

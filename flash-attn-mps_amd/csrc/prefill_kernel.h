@@ -818,9 +818,9 @@ __global__ __launch_bounds__(64 * W, MINB) void prefill_kernel(const typename At
         return e;
       };
 #pragma unroll
-      for (int it = 0; it < KIT; ++it) kbyte[it] = scale_for<T>(byte_of(0, widen_group<DQ, W>(it, wave_u)));
+      for (int it = 0; it < KIT; ++it) kbyte[it] = byte_of(0, widen_group<DQ, W>(it, wave_u));
 #pragma unroll
-      for (int it = 0; it < VIT; ++it) vbyte[it] = scale_for<T>(byte_of(1, widen_group<DV, W>(it, wave_u)));
+      for (int it = 0; it < VIT; ++it) vbyte[it] = byte_of(1, widen_group<DV, W>(it, wave_u));
     }
   };
   auto dma_fp8 = [&](int tile) {
@@ -870,7 +870,7 @@ __global__ __launch_bounds__(64 * W, MINB) void prefill_kernel(const typename At
       const int r = 4 * q + (l16 >> 2), u = 4 * g + m, rho = sigma(r), sw = (rho >> 1) & 7, up = r & 1;
       u32x4 first, second;
       widen_fp8_16<T>(halves_swapped_if(*(const u32x4*)(stk + r * DQ + 16 * (u ^ stage_rows<DQ>(r))), up), first,
-                      second, BLOCK ? e8m0_to_f32(kbyte[BLOCK ? it : 0]) : 1.0f);
+                      second, BLOCK ? e8m0_to_f32(scale_for<T>(kbyte[BLOCK ? it : 0])) : 1.0f);
       char* const row = kbuf0 + buf * KTILE + g * PF_GROUP_BYTES + rho * 128;
       *(u32x4*)(row + ((2 * m + up) ^ sw) * 16) = first;
       *(u32x4*)(row + ((2 * m + 1 - up) ^ sw) * 16) = second;
@@ -885,7 +885,7 @@ __global__ __launch_bounds__(64 * W, MINB) void prefill_kernel(const typename At
       const int r = 4 * ((it * GPI + (t >> 4)) / NC) + (l16 >> 2);
       u32x4 first, second;
       widen_fp8_16<T>(halves_swapped_if(*(const u32x4*)(stage + r * DV + 16 * (u ^ stage_rows<DV>(r))), up), first,
-                      second, BLOCK ? e8m0_to_f32(vbyte[BLOCK ? it : 0]) : 1.0f);
+                      second, BLOCK ? e8m0_to_f32(scale_for<T>(vbyte[BLOCK ? it : 0])) : 1.0f);
       char* const dst = vbuf0 + buf * VTILE + blk * PF_VBLOCK_BYTES + r * 64 + 32 * h;
       *(u32x4*)(dst + 16 * up) = first;
       *(u32x4*)(dst + 16 * (1 - up)) = second;
