@@ -4,9 +4,9 @@
 // finite run again by block_row.
 //
 // A value times its power of two is exact in bf16, and in fp16 to fp16's own
-// range; blocks past a type's range count as NaN (scale_for).  The E4M3 tiles widen every key tile again for each block of query
-// rows; with many rows a key that costs more than this pass, which HBM bounds: 3
-// bytes a value, 36K keys of 8 heads x 128, K and V, 221 MB: 63 us, 3.5 TB/s.  That
+// range; blocks past a type's range count as NaN (scale_for).  The E4M3 tiles widen
+// every key tile again for each block of query rows; with many rows a key that
+// costs more than this pass, which HBM bounds: 3 bytes a value, 36K keys of 8 heads x 128, K and V, 221 MB: 63 us, 3.5 TB/s.  That
 // prefill of 16 prompts (16/8 heads, 542 GFLOP): 650 us in all, 896 on the tiles.
 #include "block_row.h"
 
@@ -14,8 +14,9 @@ namespace {
 
 constexpr int TILE = 64;   // keys of a workgroup
 // Codes of a thread's piece: 8 are read at once, 16 bytes written next to its
-// neighbour's (16 codes, whose two writes interleave with the neighbours',
-// made the pass 15-20 us of 75 slower: 16 prompts of 256..4096, 16/8 heads d128).
+// neighbour's.  (16 codes, whose two writes interleave with the neighbours': 16
+// prompts of 256..4096, 16/8 heads d128 653 us in all against 642, a chunk over 16K
+// keys 317 against 309.)
 constexpr int CODES = 8;
 
 struct WideParams {
