@@ -355,3 +355,19 @@ def test_nothing_to_do(device):
     x = normal((3, 2, 64), 1, torch.float16).to(device)
     q = fa.append_paged_kvcache(x, x, cache, cache.clone(), cu[:1], used[:0], table[:0], q=x, rotary_cos=cos, rotary_sin=sin)
     assert torch.equal(q, x) and not cache.any()
+
+
+def test_rows_of_no_request(device):
+    """A batch of padding alone: nothing is written, q is copied."""
+    q, k = normal((5, 4, 64), 1, torch.bfloat16).to(device), normal((5, 2, 64), 2, torch.bfloat16).to(device)
+    codes, scale = (t.to(device) for t in random_cache(3, 16, 16, 2, 64, 3))
+    held = codes.clone(), codes.clone(), scale.clone(), scale.clone()
+    i32 = dict(dtype=torch.int32, device=device)
+    cos, sin = (t.to(device) for t in tables(4, 32))
+    for batch in (0, 2):
+        out = fa.append_paged_kvcache(k, k, held[0], held[1], torch.zeros(batch + 1, **i32), torch.full((batch,), 7, **i32),
+                                      torch.zeros(batch, 1, **i32), q=q, rotary_cos=cos, rotary_sin=sin, k_scale=held[2],
+                                      v_scale=held[3])
+        assert torch.equal(out, q)
+        for x, was in zip(held, (codes, codes, scale, scale)):
+            assert torch.equal(x.view(torch.uint8), was.view(torch.uint8))
