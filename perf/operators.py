@@ -17,7 +17,6 @@ benchmark and configurations, or generic.
 import os
 import random
 import sys
-from functools import lru_cache
 
 import torch
 
@@ -29,7 +28,6 @@ CODE, SCALE = torch.float8_e4m3fn, torch.float8_e8m0fnu
 DEVICE = "cuda"
 
 
-@lru_cache(maxsize=None)
 def _library():
     path = os.path.abspath("flash-attn-mps_amd")
     if path not in sys.path:
