@@ -3,6 +3,13 @@
 // 16-bit prefill kernels run on that, and rows that met a value that is not
 // finite run again by block_row.
 //
+// Sums past fp32: the prefill adds p v up before it divides by the sum of p, so
+// finite values of bf16's topmost scales may leave fp32's range where their mean
+// does not.  With n keys, p <= 2^8 (a running maximum moves in steps of 2^8) and
+// codes below 2^9, |sum p v| < 2^(17 + log2 n + e - 127): tiles with larger scales
+// than 2^128 allows are flagged too, and K's likewise (a score's sum over 256 dims
+// stays below 2^128 while |q| <= n).
+//
 // A value times its power of two is exact in bf16, and in fp16 to fp16's own
 // range; blocks past a type's range count as NaN (scale_for).  The E4M3 tiles widen
 // every key tile again for each block of query rows; with many rows a key that
@@ -23,11 +30,12 @@ constexpr int CODES = 8;
 struct WideParams {
   fa_block_attn a;
   uint16_t* out[2];       // [batch, capacity, heads, dim], K and V
-  int32_t* flags;         // [batch, tiles, 2]: whether a tile may hold values that are not finite
+  int32_t* flags;         // [batch, tiles, 2]: whether rows over a tile may hold sums that are not finite
   int32_t* lengths;       // [batch]: keys of a request in the workspace
   int64_t capacity;
   int32_t tiles;
   int32_t chunks[2];      // pieces of a head's row
+  uint32_t top_scale;     // the largest scale byte that cannot overflow a sum
 };
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -115,7 +123,7 @@ __global__ __launch_bounds__(256) void widen_kernel(const WideParams p) {
           if (key >= keys) continue;
           const uint32_t byte = scale_for<T>(e[n]);   // (here: the loads above are in flight together)
           const float scale = e8m0_to_f32(byte);
-          odd |= byte == 255;
+          odd |= byte > p.top_scale;   // (255, NaN, among them)
           const u32x2 x = widen4<BF16>(w[n][0], scale), y = widen4<BF16>(w[n][1], scale);
           *(u32x4*)(out + ((int64_t)key * per_key + piece) * CODES) = u32x4{x[0], x[1], y[0], y[1]};
           // NaN codes: 0x7f without the sign.
@@ -233,6 +241,8 @@ extern "C" int fa_block_wide_fwd(const fa_block_wide_args* args, void* stream) {
   p.lengths = p.flags + p.a.batch * 2 * fa_ceil_div(p.a.max_seqlen_k, TILE);
   FA_REQUIRE(p.a.max_seqlen_k >= 1, "%s: max_seqlen_k must be positive", who);
   p.tiles = (int32_t)fa_ceil_div(p.a.max_seqlen_k, TILE);
+  p.top_scale = 127 + 128 - 17;
+  for (int64_t n = 1; n < p.a.max_seqlen_k; n *= 2) --p.top_scale;
   p.chunks[0] = (int32_t)(p.a.head_dim_qk / CODES), p.chunks[1] = (int32_t)(p.a.head_dim_v / CODES);
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid((unsigned)p.tiles, (unsigned)p.a.batch, 2);

@@ -519,3 +519,20 @@ def test_wide_keys_before_every_window_are_not_read(device, wide):
                 t.view(torch.uint8)[edge, :(length - 77) % 64] = 0x7f
         out, lse = call.gpu(device, window_size=(77, 0))
         assert torch.equal(out, want) and torch.equal(lse, want_lse)
+
+
+@pytest.mark.parametrize("keys", [90, 700, 2000])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_wide_sums_past_fp32(device, wide, dim, keys):
+    """Values of one sign up to 2^127 under nearly equal weights: their sum leaves fp32's range, their mean does not."""
+    for byte, kw in ((246, {}), (244, dict(softcap=5.0)), (240, dict(window_size=(keys // 2, 0))), (238, dict(causal=False))):
+        call = Call([40, 30], [keys, 60], 64, 16, 4, 2, dim)
+        call.q = call.q * 2.0 ** -8
+        call.v = (call.v.view(torch.uint8) & 0x7f).view(CODE)
+        call.vs.view(torch.uint8).fill_(byte)
+        call.check(device, **kw)
+    assert "fa_block_wide_fwd" in wide
+
+
+def test_wide_scale_bytes(device, wide):
+    test_scale_bytes(device)
