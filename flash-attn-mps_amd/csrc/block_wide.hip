@@ -54,6 +54,14 @@ FA_DEV u32x2 widen4(uint32_t w, float scale) {
                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, true))};
 }
 
+// Request b with its length at most max_seqlen_k: the workspace holds no key past
+// that, and every part of the call has to place the rows alike.
+FA_DEV RequestInfo bounded_request(const fa_attn_args& a, int64_t b) {
+  RequestInfo r = load_request(a, b);
+  r.k_len = (int)min((int64_t)r.k_len, a.max_seqlen_k);
+  return r;
+}
+
 // The first key of request r that some query row sees.
 FA_DEV int first_key(const fa_attn_args& a, const RequestInfo& r) {
   if (a.mask_kind != 0 || a.window_left < 0) return 0;
@@ -72,11 +80,11 @@ __global__ __launch_bounds__(256) void widen_kernel(const WideParams p) {
   const fa_block_attn& a = p.a;
   const int tile = blockIdx.x, which = blockIdx.z;
   const int64_t b = blockIdx.y;
-  const RequestInfo r = load_request(a, b);
+  const RequestInfo r = bounded_request(a, b);
   const int heads = (int)a.heads_k, chunks = p.chunks[which], per_key = heads * chunks;
   const int64_t* const st = which ? a.v_stride : a.k_stride;
   const uint8_t* const in = (const uint8_t*)(which ? a.v : a.k);
-  const int begin = tile * TILE, end = min(begin + TILE, (int)min((int64_t)r.k_len, p.capacity));
+  const int begin = tile * TILE, end = min(begin + TILE, r.k_len);
   bool odd = false;
   // The prefill reads whole tiles of up to 128 keys: the first one's keys that no
   // row sees are zeros here, and their pages are not read.
@@ -135,8 +143,7 @@ __global__ __launch_bounds__(256) void widen_kernel(const WideParams p) {
   const int any = __syncthreads_or(odd);
   if (threadIdx.x != 0) return;
   p.flags[(b * p.tiles + tile) * 2 + which] = any;
-  // (A length past the caller's max_seqlen_k has no rows here.)
-  if (tile == 0 && which == 0) p.lengths[b] = (int)min((int64_t)r.k_len, p.capacity);
+  if (tile == 0 && which == 0) p.lengths[b] = r.k_len;
 }
 
 // Rows whose output is not finite, where some tile was flagged: a few workgroups
@@ -150,7 +157,7 @@ __global__ __launch_bounds__(256) void again_kernel(const WideParams p) {
   if (!__syncthreads_or(odd)) return;
   const int Dv = (int)a.head_dim_v;
   for (int64_t b = 0; b < a.batch; ++b) {
-    const RequestInfo r = load_request(a, b);
+    const RequestInfo r = bounded_request(a, b);
     if (!runs_here(a, r)) continue;
     for (int64_t i = (int64_t)blockIdx.x * 4 + wave; i < (int64_t)r.q_len * a.heads_q; i += (int64_t)gridDim.x * 4) {
       const int row = (int)(i / a.heads_q), h = (int)(i - (int64_t)row * a.heads_q);

@@ -536,3 +536,19 @@ def test_wide_sums_past_fp32(device, wide, dim, keys):
 
 def test_wide_scale_bytes(device, wide):
     test_scale_bytes(device)
+
+
+@pytest.mark.parametrize("more", [20, 200])
+@pytest.mark.parametrize("dim", [64, 128, 256, 80])
+def test_wide_length_past_the_callers_maximum_behind_a_window(device, wide, dim, more):
+    """As with a length of max_seqlen_k: the rows' places, the keys that they see, and the rows that meet a NaN."""
+    for kw in (dict(window_size=(50, 0)), dict(window_size=(9, 0), softcap=5.0)):
+        call = Call([40, 30], [90, 400], 64, 16, 4, 2, dim)
+        call.v.view(torch.uint8)[int(call.table[1, 5]), 60, 1, 5] = 0x7f    # key 380: rows 10 and on
+        want, want_lse = call.gpu(device, **kw)
+        call.used[1] = 400 + more
+        call.table = torch.nn.functional.pad(call.table, (0, 4), value=0)
+        out, lse = call.gpu(device, max_k=400, **kw)
+        bits = lambda t: t.view(torch.int16)  # noqa: E731
+        assert torch.equal(bits(out), bits(want)) and torch.equal(lse, want_lse)
+        assert out[50:60, 2:, 5].isnan().all() and not out[:50].isnan().any() and not out[:, :2].isnan().any()
