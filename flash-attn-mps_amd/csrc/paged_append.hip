@@ -270,14 +270,14 @@ FA_DEV Piece<W> narrow(const float (&f)[W]) {
   }
 }
 
-// a x - b y.  TIES: the rounding of b y goes back in (a large number where
-// there is none, b y being infinite), since ties between E4M3 codes are where
-// rounding twice shows: of 20M rotated values 14 codes off the 64-bit ones, 20
-// without it and 32 with each product rounded.
+// a x - b y.  TIES: the rounding of b y goes back in (bounded to either side: where
+// b y is infinite there is none, and the difference stays infinite), since ties
+// between E4M3 codes are where rounding twice shows: of 20M rotated values 14 codes
+// off the 64-bit ones, 20 without it and 32 with each product rounded.
 template <bool TIES>
 FA_DEV float turned_by(float a, float x, float b, float y) {
   const float by = b * y, v = fmaf(a, x, -by);
-  return TIES ? v + fminf(fmaf(-b, y, by), 3e38f) : v;
+  return TIES ? v + __builtin_amdgcn_fmed3f(fmaf(-b, y, by), -3e38f, 3e38f) : v;
 }
 
 // The W pairs of a unit turned; lo and hi are its pieces.

@@ -371,3 +371,37 @@ def test_rows_of_no_request(device):
         assert torch.equal(out, q)
         for x, was in zip(held, (codes, codes, scale, scale)):
             assert torch.equal(x.view(torch.uint8), was.view(torch.uint8))
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rotated_overflows_saturate(device, interleaved, dtype):
+    """Finite keys whose rotation leaves fp32's range, to either side: infinities, as those of infinite keys.
+
+    Tables of magnitude 1.5 (scaled rotary embeddings) and keys of 3e38: a product of 4.5e38 overflows, and its pair's
+    other key is 1, so each result is one such product, its sign that of the formula."""
+    x = normal((20, 2, 64), 5, dtype)
+    big = torch.tensor(3e38).to(dtype)
+    cos, sin = (t * 1.5 for t in tables(20, 16))
+    angle = torch.where(torch.arange(16) % 2 == 0, 1.0, -1.0).expand(20, 16)     # sin = +-1.5 cos = 0
+    cos[10:], sin[10:] = 0.0, 1.5 * angle[10:]
+    for row, pair, high, sign in ((12, 4, False, 1), (13, 5, False, 1), (14, 4, True, 1), (15, 5, True, 1), (16, 4, True, -1), (17, 5, False, -1)):
+        lo, hi = (2 * pair, 2 * pair + 1) if interleaved else (pair, pair + 16)
+        x[row, 1, lo], x[row, 1, hi] = (1.0, sign * big) if high else (sign * big, 1.0)
+    cu, used = torch.tensor([0, 20], dtype=torch.int32), torch.tensor([20], dtype=torch.int32)
+    table = torch.tensor([[2, 0]], dtype=torch.int32)
+    turned = rotate(x, cos, sin, torch.arange(20)[None], None, interleaved).float().double()     # 4.5e38: infinite
+    assert turned.isinf().sum() == 6 and not turned.isnan().any()
+    for scales in ("block", "head"):
+        codes, scale = random_cache(3, 16, 16, 2, 64, 3)
+        cache, got_scale = codes.to(device), scale.to(device) if scales == "block" else torch.ones(2, device=device)
+        fa.append_paged_kvcache(x.to(device), x.to(device), cache, cache.clone(), cu.to(device), used.to(device), table.to(device),
+                                rotary_cos=cos.to(device), rotary_sin=sin.to(device), rotary_interleaved=interleaved,
+                                k_scale=got_scale, v_scale=got_scale.clone())
+        if scales == "block":
+            code, factor = append(codes, scale, turned, cu, used, table)
+            assert torch.equal(scale_values(got_scale), factor)
+        else:
+            code = codes.double()
+            code[2], code[0, :4] = encode(turned[:16]), encode(turned[16:])
+        assert_codes(cache, code, False)
