@@ -30,8 +30,9 @@ BLOCK_SCALE = torch.float8_e8m0fnu
 
 
 def is_block_scale(scale):
-    """Whether `scale` is the scales of a block-scaled cache (E8M0, a power of two per block and head)."""
-    return torch.is_tensor(scale) and scale.dtype == BLOCK_SCALE
+    """Whether `scale` is the scales of a block-scaled cache: E8M0 [pages, blocks, heads], a power of two per block
+    and head.  (E8M0 tensors of fewer dims are values like any others: one, or one per head.)"""
+    return torch.is_tensor(scale) and scale.dtype == BLOCK_SCALE and scale.ndim > 2
 
 
 def block_of(cache, scale, name):

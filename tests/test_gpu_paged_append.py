@@ -405,3 +405,18 @@ def test_rotated_overflows_saturate(device, interleaved, dtype):
             code = codes.double()
             code[2], code[0, :4] = encode(turned[:16]), encode(turned[16:])
         assert_codes(cache, code, False)
+
+
+def test_e8m0_scales_per_head(device):
+    """E8M0 values in place of fp32 ones, for a slot write and an append: the same codes."""
+    k, v = (normal((5, 2, 64), i, torch.bfloat16).to(device) for i in (1, 2))
+    scale = torch.tensor([120, 125], dtype=torch.uint8, device=device).view(SCALE)
+    i32 = dict(dtype=torch.int32, device=device)
+    got = []
+    for s in (scale, scale.float()):
+        caches = [torch.zeros(2, 16, 2, 64, device=device).to(CODE) for _ in range(4)]
+        fa.store_kvcache(k, v, caches[0], caches[1], torch.arange(3, 8, device=device), k_scale=s, v_scale=s[1:])
+        fa.append_paged_kvcache(k, v, caches[2], caches[3], torch.tensor([0, 5], **i32), torch.tensor([8], **i32),
+                                torch.zeros(1, 1, **i32), k_scale=s, v_scale=s[1:])
+        got.append(torch.stack([c.view(torch.uint8) for c in caches]))
+    assert torch.equal(*got) and torch.equal(got[0][:2], got[0][2:])

@@ -235,3 +235,20 @@ def test_wide_entry_refuses_null_and_mismatched_arguments():
     assert lib.fa_block_wide_fwd(ctypes.byref(a), None) == 1
     a.size = ctypes.sizeof(a)
     assert lib.fa_block_wide_fwd(ctypes.byref(a), None) == 1 and not _lib.supported("fa_block_wide_supported", a)
+
+
+@pytest.mark.parametrize("shape,stride", [((), 0), ((1,), 0), ((2,), 1), ((1, 2), 1)])
+def test_slot_writes_take_e8m0_values(shape, stride):
+    """One value, or one per head, converts whatever its type; three dims are scales per block."""
+    scale = torch.full(shape, 124, dtype=torch.uint8).view(SCALE)
+    got, step = _cache._per_head_scale(scale, 2, torch.device("cpu"))
+    assert got.dtype == torch.float32 and (got == 0.125).all() and got.numel() == 1 + stride and step == stride
+
+
+def test_append_takes_e8m0_values_as_scales_per_head(launches):
+    scale = torch.tensor([124, 130], dtype=torch.uint8).view(SCALE)
+    paged(k_scale=scale, v_scale=scale[:1])
+    args = launches[0][1]
+    assert args.block == 0 and [d.scale_stride for d in args.kv] == [1, 0]
+    with pytest.raises(ValueError, match="one per KV head"):
+        paged(k_scale=torch.zeros(5, 2, dtype=torch.uint8).view(SCALE), v_scale=None)
