@@ -153,8 +153,8 @@ _WIDE_BYTES = 4 << 30
 def takes_prefill(p, a):
     """Whether the MFMA prefill takes arguments `a` of Problem `p`, by way of
     16-bit rows (p.wide then holds the workspace) for block-scaled caches where
-    that pays or the tiles do not.  Calls with a fixed order stay on the tiles,
-    whose choice does not depend on the batch."""
+    that pays or the tiles do not, and memory for it is there.  Calls with a fixed
+    order stay on the tiles, whose choice does not depend on the batch."""
     if not p.block_scaled:
         return _lib.supported("fa_prefill_supported", a)
     rows, visible = p.tokens / p.batch, p.visible_max
@@ -167,9 +167,12 @@ def takes_prefill(p, a):
     if tiles or p.deterministic or not 0 < size <= _WIDE_BYTES or p.q.dtype == torch.float8_e4m3fn:
         return tiles or (pays and supported(p, "fa_prefill_supported", a))
     from .interface import _counting
-    identity = _counting.rows(p.batch, p.device)
-    work = torch.empty(size // 2, dtype=p.q.dtype, device=p.device)
-    flags = torch.empty(p.batch * (2 * -(-p.max_k // 64) + 1), dtype=torch.int32, device=p.device)
+    try:
+        identity = _counting.rows(p.batch, p.device)
+        work = torch.empty(size // 2, dtype=p.q.dtype, device=p.device)
+        flags = torch.empty(p.batch * (2 * -(-p.max_k // 64) + 1), dtype=torch.int32, device=p.device)
+    except torch.OutOfMemoryError:   # (a cache that fills the GPU: the tiles need no workspace)
+        return pays and supported(p, "fa_prefill_supported", a)
     p.wide = (work.data_ptr(), work.data_ptr() + 2 * keys * p.dim_qk, p.max_k, identity.data_ptr(), flags.data_ptr())
     if supported(p, "fa_prefill_supported", a):
         p.keep += [identity, work, flags]

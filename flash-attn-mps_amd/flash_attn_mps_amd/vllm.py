@@ -76,6 +76,9 @@ def flash_attn_varlen_func(
     ``append_paged_kvcache`` fills it, float8_e8m0fnu [pages, page_size / block, Hkv]:
     a power of two per block of tokens and head, in place of descales.  With float16
     queries the cache's values enter products as float16 (below 2^-25 as zeros).
+    Prompts over such a cache take a workspace for the call, 2 x requests x
+    max_seqlen_k x Hkv x (Dqk + Dv) bytes (a captured graph keeps it); without that
+    memory, or past 4 GiB, they run without it, more slowly.
     """
     reject_training(dropout_p, return_attn_probs, (q, k, v))
     if fa_version not in (2, 3, 4):

@@ -552,3 +552,18 @@ def test_wide_length_past_the_callers_maximum_behind_a_window(device, wide, dim,
         bits = lambda t: t.view(torch.int16)  # noqa: E731
         assert torch.equal(bits(out), bits(want)) and torch.equal(lse, want_lse)
         assert out[50:60, 2:, 5].isnan().all() and not out[:50].isnan().any() and not out[:, :2].isnan().any()
+
+
+def test_no_memory_for_a_workspace(device, wide, monkeypatch):
+    """The tiles run, or the generic kernel for what they do not take."""
+    empty = torch.empty
+
+    def short_of_memory(*size, **kw):
+        if kw.get("dtype") == torch.bfloat16 and isinstance(size[0], int):
+            raise torch.OutOfMemoryError("out of memory")
+        return empty(*size, **kw)
+
+    monkeypatch.setattr(torch, "empty", short_of_memory)
+    Call([40, 1], [90, 300], 64, 16, 4, 2, 128).check(device)
+    Call([40, 1], [90, 300], 64, 16, 4, 2, 96).check(device)
+    assert wide[-1] == "fa_block_attn_fwd" and "fa_block_prefill_fwd" in wide and "fa_block_wide_fwd" not in wide

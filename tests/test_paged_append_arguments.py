@@ -252,3 +252,27 @@ def test_append_takes_e8m0_values_as_scales_per_head(launches):
     assert args.block == 0 and [d.scale_stride for d in args.kv] == [1, 0]
     with pytest.raises(ValueError, match="one per KV head"):
         paged(k_scale=torch.zeros(5, 2, dtype=torch.uint8).view(SCALE), v_scale=None)
+
+
+@pytest.mark.parametrize("dim,route", [(128, "tiles"), (96, "generic")])
+def test_attention_without_memory_for_a_workspace(monkeypatch, dim, route):
+    """A workspace that cannot be had leaves a prefill to the tiles, or to the generic kernel."""
+    from flash_attn_mps_amd import _attention
+    from flash_attn_mps_amd._problem import Problem
+    codes = torch.zeros(4, 64, 2, dim).to(CODE)
+    scale = torch.zeros(4, 4, 2, dtype=torch.uint8).view(SCALE)
+    q = torch.zeros(128, 32, dim, dtype=torch.bfloat16)
+    p = Problem(q, codes, codes.clone(), torch.tensor([0, 128], dtype=torch.int32), 128, 200,
+                used_k=torch.tensor([200], dtype=torch.int32), table=torch.zeros(1, 4, dtype=torch.int32), causal=True,
+                k_descale=scale, v_descale=scale.clone())
+    a = _attention.build_args(p, torch.empty_like(q), torch.empty(32, 128))
+    assert _attention.takes_prefill(p, a) and p.wide is not None
+    p.wide, empty = None, torch.empty
+
+    def short_of_memory(*size, **kw):
+        if size[0] >= 200 * 2 * dim:
+            raise torch.OutOfMemoryError("out of memory")
+        return empty(*size, **kw)
+
+    monkeypatch.setattr(torch, "empty", short_of_memory)
+    assert _attention.takes_prefill(p, a) == (route == "tiles") and p.wide is None
