@@ -567,3 +567,84 @@ def test_no_memory_for_a_workspace(device, wide, monkeypatch):
     Call([40, 1], [90, 300], 64, 16, 4, 2, 128).check(device)
     Call([40, 1], [90, 300], 64, 16, 4, 2, 96).check(device)
     assert wide[-1] == "fa_block_attn_fwd" and "fa_block_prefill_fwd" in wide and "fa_block_wide_fwd" not in wide
+
+
+@pytest.mark.parametrize("lengths", [[128, 90], [2100, 1500]])
+@pytest.mark.parametrize("dim", [128, 256, 80])
+def test_wide_not_finite_beside_features(device, wide, dim, lengths):
+    """A NaN in a key, then in a value, of one KV head, with softcap, windows and (long keys) key splits: the rows that
+    see it, their heads, the value's dim alone; all else at the bar of the same call without it.  Not bit for bit, as in
+    test_nan_reaches_the_rows_that_see_it."""
+    rows, at = 64, lengths[0] - 64 + 17          # row 17's own key
+    for kw in ({}, dict(softcap=5.0), dict(window_size=(30, 0)), dict(softcap=5.0, window_size=(30, 0)), dict(causal=False)):
+        sees = torch.arange(rows) >= (0 if kw.get("causal") is False else 17)
+        if "window_size" in kw:
+            sees &= torch.arange(rows) <= 17 + 30
+        base = Call([rows, 40], lengths, 64, 16, 8, 4, dim)
+        want, want_lse = base.gpu(device, **kw)
+        for which in ("k", "v"):
+            call = Call([rows, 40], lengths, 64, 16, 8, 4, dim)
+            getattr(call, which).view(torch.uint8)[int(call.table[0, at // 64]), at % 64, 1, 5] = 0xff
+            out, lse = call.gpu(device, **kw)
+            nan = torch.zeros(rows + 40, 8, dim, dtype=torch.bool)
+            nan[:rows, 2:4][sees] = True
+            if which == "v":
+                nan[..., :5] = nan[..., 6:] = False
+            assert torch.equal(out.isnan().cpu(), nan)
+            keep = ~nan
+            assert ((out.cpu() - want.cpu()).abs() <= OUT_BAR[torch.bfloat16])[keep].all()
+            clean = ~nan.any(-1).T if which == "k" else torch.ones(8, rows + 40, dtype=torch.bool)
+            assert ((lse.cpu() - want_lse.cpu()).abs() <= 1e-4)[clean].all() and torch.isneginf(lse.cpu()[~clean]).all()
+    assert "fa_block_wide_fwd" in wide
+
+
+@pytest.mark.parametrize("dim", [64, 256])
+@pytest.mark.parametrize("lengths", [[200, 90], [1800, 1200]])
+def test_wide_beyond_16_bits_beside_features(device, wide, dim, lengths):
+    """Keys and values past the 16-bit type's range with softcap, windows and key splits: as beyond_16_bits."""
+    for dtype in (torch.float16, torch.bfloat16):
+        byte = 127 + (10 if dtype == torch.float16 else 120)
+        for kw in ({}, dict(softcap=5.0), dict(softcap=5.0, window_size=(180, 0))):
+            for which in ("k", "v")[dtype == torch.bfloat16:]:
+                call = Call([70, 30], lengths, 64, 16, 4, 2, dim, dtype)
+                codes, scales = (call.k, call.ks) if which == "k" else (call.v, call.vs)
+                page, block = int(call.table[0, (lengths[0] - 60) // 64]), (lengths[0] - 60) % 64 // 16
+                codes.view(torch.uint8)[page, 16 * block:16 * block + 16, 1] = 0
+                codes.view(torch.uint8)[page, 16 * block + 4, 1, 7] = 0x7e
+                scales.view(torch.uint8)[page, block, 1] = byte
+                call.q[:, 2:, 7] = -2.0 ** -16
+                call.check(device, **kw)
+    assert "fa_block_wide_fwd" in wide
+
+
+def scales_apart(device, rows, low, spread, dtype, dim, **kw):
+    """As test_wide_scales, each output held to its own sum p |v|: rows, heads and dims of small blocks too.  Beside that
+    only the types' smallest steps: 2^-24 in fp16 (values and outputs, half a step each), 2^-132 in bf16."""
+    call = Call([rows, 3], [200, 90], 64, 16, 4, 2, dim, dtype)
+    _, call.vs = random_cache(call.v.shape[0], 64, 16, 2, dim, 77, low, spread)
+    out, lse = call.gpu(device, **kw)
+    ref, ref_lse = call.oracle(**kw)
+    call.v = (call.v.view(torch.uint8) & 0x7f).view(CODE)
+    bar = 2 * HALF_STEP[dtype] * call.oracle(**kw)[0] * (1 + 2.0 ** -5) + (2.0 ** -24 if dtype == torch.float16 else 2.0 ** -132)
+    off = (out.cpu().double() - ref).abs()
+    assert (off <= bar).all(), f"off by up to {(off / bar).max():.3f} of the tolerance"
+    assert ((lse.cpu().double() - ref_lse).abs().max() <= 1e-4).item()
+
+
+APART = [(-40, 3, torch.bfloat16), (20, 3, torch.bfloat16), (-15, 8, torch.float16), (-60, 60, torch.bfloat16)]
+
+
+@pytest.mark.parametrize("rows", [1, 3, 70])
+@pytest.mark.parametrize("low,spread,dtype", APART)
+def test_scales_apart(device, rows, low, spread, dtype):
+    scales_apart(device, rows, low, spread, dtype, 128)
+    scales_apart(device, rows, low, spread, dtype, 64, window_size=(20, 0))
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256, 80])
+@pytest.mark.parametrize("low,spread,dtype", APART)
+def test_wide_scales_apart(device, wide, low, spread, dtype, dim):
+    scales_apart(device, 70, low, spread, dtype, dim)
+    scales_apart(device, 70, low, spread, dtype, dim, window_size=(20, 0))
+    scales_apart(device, 70, low, spread, dtype, dim, window_size=(0, 0))
+    assert "fa_block_wide_fwd" in wide
