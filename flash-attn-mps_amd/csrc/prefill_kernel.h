@@ -1722,8 +1722,10 @@ PrefillChoiceOf<fa_block_attn> pick_tile_block(bool cap, bool win, int mk, bool 
     }
   } else if (split) {
     if (win) return c;
-    c.kern = cap ? prefill_kernel<T, DQ, DV, S::W, S::NB, S::MINB, CAUSAL, true, false, DQ, DV, E4M3T, false, T, 0, true, true>
-                 : prefill_kernel<T, DQ, DV, S::W, S::NB, S::MINB, CAUSAL, false, false, DQ, DV, E4M3T, false, T, 0, true, true>;
+    if constexpr (DQ <= 128) {   // (split_ok: softcap at 64 and 128 dims)
+      if (cap) c.kern = prefill_kernel<T, DQ, DV, S::W, S::NB, S::MINB, CAUSAL, true, false, DQ, DV, E4M3T, false, T, 0, true, true>;
+    }
+    if (!cap) c.kern = prefill_kernel<T, DQ, DV, S::W, S::NB, S::MINB, CAUSAL, false, false, DQ, DV, E4M3T, false, T, 0, true, true>;
   } else if (win) {
     c.kern = cap ? prefill_kernel<T, DQ, DV, S::W, S::NB, S::MINB_WIN, CAUSAL, true, true, DQ, DV, E4M3T, false, T, 0, false, true>
                  : prefill_kernel<T, DQ, DV, S::W, S::NB, S::MINB_WIN, CAUSAL, false, true, DQ, DV, E4M3T, false, T, 0, false, true>;
