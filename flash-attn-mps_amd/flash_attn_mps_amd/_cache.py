@@ -54,10 +54,21 @@ def _require_gpu(**tensors):
             raise ValueError(f"{name} is on {t.device}; cache operations run on a ROCm GPU")
 
 
-@lru_cache(maxsize=None)
+_ONES = {}
+
+
 def _one(device):
-    """A resident fp32 1.0 per device: the FP8 scale when the caller gives none."""
-    return torch.ones(1, dtype=torch.float32, device=device)
+    """A resident fp32 1.0 per device: the FP8 scale when the caller gives none.
+    Copied from the host, so that no other stream can find it unwritten; one made
+    while a graph is captured is written by its replays, and stays that call's own."""
+    one = _ONES.get(device)
+    if one is None:
+        if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            return torch.ones(1, dtype=torch.float32, device=device)
+        one = torch.ones(1, dtype=torch.float32, device="cpu").to(device)
+        if type(one) is torch.Tensor:   # (not a tracer's stand-in)
+            _ONES[device] = one
+    return one
 
 
 def _per_head_scale(scale, heads, device):

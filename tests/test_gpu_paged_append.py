@@ -420,3 +420,23 @@ def test_e8m0_scales_per_head(device):
                                 torch.zeros(1, 1, **i32), k_scale=s, v_scale=s[1:])
         got.append(torch.stack([c.view(torch.uint8) for c in caches]))
     assert torch.equal(*got) and torch.equal(got[0][:2], got[0][2:])
+
+
+def test_default_scale_made_in_a_capture(device, monkeypatch):
+    """An append without scales, captured first: the eager calls before the graph's first replay do not read what it writes."""
+    from flash_attn_mps_amd import _cache
+    monkeypatch.setattr(_cache, "_ONES", {}, raising=False)
+    x = normal((5, 2, 64), 1, torch.bfloat16)
+    rows = x.to(device)
+    cu, used, table = (torch.tensor(t, dtype=torch.int32, device=device) for t in ([0, 5], [5], [[0]]))
+    caches = [torch.zeros(1, 16, 2, 64, device=device).to(CODE) for _ in range(4)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        fa.append_paged_kvcache(rows, rows, caches[0], caches[1], cu, used, table)
+    fa.append_paged_kvcache(rows, rows, caches[2], caches[3], cu, used, table)
+    torch.cuda.synchronize()
+    for got in (caches[2:], caches):
+        for c in got:
+            assert torch.equal(c[0, :5].cpu().double(), encode(x.double()))
+        graph.replay()
+        torch.cuda.synchronize()
