@@ -20,7 +20,8 @@ FA_DEV const fa_block_attn& block_arguments() {
 
 // q(d): the query's element d.  emit(d, x): output element d, normalised.  The
 // row sees keys of [begin, end) that key_allowed lets through; the sink joins
-// split 0.  Returns the LSE: -inf without a key, NaN where the sum is.
+// split 0.  Returns the LSE: -inf without a key, NaN where the sum is.  Values
+// enter the sum times 2^-16, so that 2^16 keys of the largest stay in fp32.
 // Dv <= 64 * ACC.
 template <int ACC, typename Q, typename E>
 FA_DEV float block_row(const fa_block_attn& a, int64_t b, const RequestInfo& r, int kh, int h, int split, int64_t tq,

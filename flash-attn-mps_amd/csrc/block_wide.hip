@@ -13,9 +13,9 @@
 // A value times its power of two is exact in bf16, and in fp16 to fp16's own
 // range; blocks past a type's range count as NaN (scale_for).  The E4M3 tiles widen
 // every key tile again for each block of query rows; with many rows a key that
-// costs more than this pass, which HBM bounds: 3 bytes a value, 36K keys of 8 heads
-// x 128, K and V, 221 MB: 63 us, 3.5 TB/s.  That prefill of 16 prompts (16/8 heads,
-// 542 GFLOP): 650 us in all, 896 on the tiles.
+// costs more than this pass, which HBM bounds: 3 bytes a value, 43K keys of 8 heads
+// x 128, K and V, 264 MB: 56 us, 4.7 TB/s.  That prefill of 16 prompts (16/8 heads,
+// 542 GFLOP): 669 us in all, 901 on the tiles, 614 on a 16-bit cache.
 #include "block_row.h"
 
 namespace {

@@ -25,8 +25,8 @@
 // turned, 8 do as they came).
 //
 // Kernel times: 9001 tokens of 16 + 16 heads d80 on two axes, 94 MB: 26.6 us, 3.5
-// TB/s; 4100 rows of 16 + 4 + 4 heads d256 to a 16-bit cache, 103 MB: 23.6 us, 4.4
-// TB/s; 36K rows of 16 + 8 + 8 heads d128 to a block-scaled one, 619 MB: 150 us, 4.1
+// TB/s; 4095 rows of 16 + 4 + 4 heads d256 to a 16-bit cache, 103 MB: 23.6 us, 4.4
+// TB/s; 43K rows of 16 + 8 + 8 heads d128 to a block-scaled one, 619 MB: 149 us, 4.2
 // TB/s (a large copy: 4.8); one token: 4.0 us, with its append 5.9.
 #include "attn_common.h"
 
@@ -462,7 +462,7 @@ FA_DEV int block_exponent(float most) {
 }
 
 // Rows a lane holds between a block's largest magnitude and its codes.  GPU us with
-// 2 / 4 / 8: 36K rows, blocks of 32, 157.4 / 147.4 / 146.3; 64 requests of one row,
+// 2 / 4 / 8: 43K rows, blocks of 32, 157.4 / 147.4 / 146.3; 64 requests of one row,
 // blocks of 16, 5.7 / 5.7 / 6.3.
 constexpr int HOLD = 4;
 

@@ -400,8 +400,8 @@ FA_DEV void rows_again(uint32_t bad, int64_t b, const RequestInfo& r, int kh, in
 // take that group's power of two into the conversion at no cost; its bytes are
 // loaded a tile ahead, with the codes.  Rows whose sums are not finite (a NaN in
 // a value that another row of the tile sees; a block past T's range) run again by
-// block_row.  16 prompts of 256..4096, 16/8 heads d128: 896 us, 605 TFLOP/s; the
-// widening of every tile is what it spends beside the 16-bit kernel's 608 us.
+// block_row.  16 prompts of 256..4096, 16/8 heads d128: 901 us, 602 TFLOP/s; the
+// widening of every tile is what it spends beside the 16-bit kernel's 614 us.
 // SPLIT: a.num_splits workgroups (blockIdx.y; request_splits of them at work)
 // share each work item's key tiles evenly and write fp32 partials for
 // prefill_merge_kernel: for grids that leave CUs idle (a chunk of a few hundred

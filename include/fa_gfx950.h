@@ -275,7 +275,8 @@ typedef struct fa_block_attn_args {
 
 /* The same by way of 16-bit rows: the keys and values that the rows see are
  * widened to the queries' type into a workspace, and the 16-bit prefill runs on
- * that (its partials and splits in block.attn). */
+ * that (its partials and splits in block.attn).  A length past max_seqlen_k counts
+ * as max_seqlen_k. */
 typedef struct fa_block_wide_args {
   int64_t size;                /* sizeof(fa_block_wide_args) */
   fa_block_attn_args block;
